@@ -384,6 +384,101 @@ int isp_conv1d_dynamic_noalloc(const void *x, int x_dtype, int64_t B, int C, int
                                int64_t T_out, const float *w_scale, const float *bias, void *y,
                                int out_dtype, isp_stream_t stream);
 
+/*
+ * Paged key-value cache of one attention layer (no reference counterpart as a call: the
+ * reference keeps contiguous 16-bit caches inside its engines, e.g. the append of
+ * ops/triton/target_kv_write.py).
+ *
+ * k, v:     [pages, kv_heads, page_size, head_dim] in dtype ISP_BF16, ISP_F16, ISP_E4M3 or
+ *           ISP_I8, contiguous, 16-byte aligned; head_dim 64 or 128, page_size >= 1,
+ *           pages * kv_heads * page_size <= 2^32 - 1.
+ * k_scale, v_scale: FP32 [pages, kv_heads, page_size] for the 8-bit types, else NULL:
+ *           s = max(amax / Q, 1e-12) of each row (Q = 448 E4M3, 127 INT8),
+ *           code = RNE(x / s), every step rounded in FP32 (the rule of ISP_Q_E4M3_ROW).
+ *           A row with a non-finite element gets scale NaN and codes 0.
+ *
+ * page_table: int32 [B, >= table_width], row stride table_stride elements: the page that
+ *           holds positions [j * page_size, (j + 1) * page_size) of sequence b is
+ *           page_table[b][j].  lengths: int32 [B], tokens of each sequence, those of this
+ *           call included.  cu_seqlens: int32 [B + 1], ascending from 0: the call's tokens
+ *           of sequence b are rows [cu[b], cu[b + 1]); NULL means one token per sequence
+ *           (T == B).  Token i of sequence b's n tokens has position lengths[b] - n + i; a
+ *           negative position is no token (nothing written, zeros read).
+ * These arrays are device memory and are read by the kernels, so a page id outside
+ * [0, pages), a length beyond table_width * page_size or a cu_seqlens outside its rows
+ * cannot be refused by the call: the kernel skips what it names and records ISP_ERR_ARG in
+ * the device error word (isp_read_device_error).
+ *
+ * Every array these calls read may be the output of the preceding call on the stream.
+ */
+typedef struct isp_kv_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t pages;
+  int32_t dtype, page_size, kv_heads, head_dim;
+} isp_kv_cache_t;
+
+/* Write T rows of K and V into the cache, quantised on the way.  k, v: [T, kv_heads,
+   head_dim] in x_dtype (ISP_BF16, ISP_F16, ISP_F32), the last dimension contiguous, the
+   other strides in elements, each a multiple of 16 bytes (16-byte aligned base).  Two
+   tokens of one call must not name the same cache row. */
+int isp_kv_append(const void *k, const void *v, int x_dtype, int64_t T,
+                  int64_t k_token_stride, int64_t k_head_stride,
+                  int64_t v_token_stride, int64_t v_head_stride,
+                  const int32_t *cu_seqlens, const int32_t *page_table, int64_t table_stride,
+                  int table_width, const int32_t *lengths, int B,
+                  const isp_kv_cache_t *cache, isp_stream_t stream);
+
+/* Read T rows back: code * scale (one FP32 product) rounded to out_dtype (ISP_BF16,
+   ISP_F16, ISP_F32).  k_out, v_out: [T, kv_heads, head_dim] contiguous.  With cu_seqlens
+   the running sum of `lengths` this unpages whole sequences, e.g. as the keys of
+   isp_prompt_attention. */
+int isp_kv_gather(const isp_kv_cache_t *cache, const int32_t *cu_seqlens,
+                  const int32_t *page_table, int64_t table_stride, int table_width,
+                  const int32_t *lengths, int B, int64_t T, int out_dtype,
+                  void *k_out, void *v_out, isp_stream_t stream);
+
+/*
+ * Attention of packed sequences: out = softmax(scale * q k^T) v per sequence and head,
+ * query head h with key head h / (heads / kv_heads).  Query i of sequence b's n sees its m
+ * keys all (causal = 0) or keys j <= i + m - n (causal = 1: the last query sees the last
+ * key); a query that sees no key gets zeros.  Masked keys and values are not read into the
+ * result whatever they hold.
+ *
+ * q: [q_tokens, heads, head_dim], k, v: [k_tokens, kv_heads, head_dim] in `dtype` (ISP_BF16
+ * or ISP_F16), out like q in the same type; strides in elements as in isp_kv_append.
+ * cu_seqlens_q, cu_seqlens_k: int32 [B + 1] device arrays as above.  head_dim 64 or 128,
+ * heads % kv_heads == 0, scale finite and positive.
+ */
+int isp_prompt_attention(const void *q, const void *k, const void *v, int dtype,
+                         int64_t q_tokens, int64_t k_tokens,
+                         const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int B,
+                         int heads, int kv_heads, int head_dim,
+                         int64_t q_token_stride, int64_t q_head_stride,
+                         int64_t k_token_stride, int64_t k_head_stride,
+                         int64_t v_token_stride, int64_t v_head_stride,
+                         float scale, int causal, void *out,
+                         int64_t out_token_stride, int64_t out_head_stride,
+                         isp_stream_t stream);
+
+/*
+ * Attention of one token per sequence over the paged cache: q, out: [B, heads, head_dim] in
+ * `dtype` (ISP_BF16 or ISP_F16), strides as above; the token sees positions
+ * [0, lengths[b]) (its own row is appended before); length 0 gives zeros.  A 16-bit cache
+ * has q's type.
+ *
+ * workspace: isp_paged_decode_workspace bytes of device memory, 256-byte aligned, zero
+ * before its first use; every call leaves it ready for the next one on the same stream.
+ * Calls that may overlap in time need a workspace each.
+ */
+int isp_paged_decode_workspace(int64_t *bytes);
+int isp_paged_decode(const void *q, int dtype, int64_t q_seq_stride, int64_t q_head_stride,
+                     const isp_kv_cache_t *cache, const int32_t *page_table,
+                     int64_t table_stride, int table_width, const int32_t *lengths, int B,
+                     int heads, float scale, void *out, int64_t out_seq_stride,
+                     int64_t out_head_stride, void *workspace, int64_t workspace_bytes,
+                     isp_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

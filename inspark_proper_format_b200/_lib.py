@@ -20,6 +20,16 @@ Q_E4M3_STATIC, Q_E4M3_ROW, Q_INT8_STATIC, Q_NVFP4, Q_NVFP4_MMA = range(5)
 
 _vp, _i, _i64, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
+
+class KVCache(ctypes.Structure):
+    """``isp_kv_cache_t`` of include/isp_b200.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64),
+                ("dtype", ctypes.c_int32), ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
+_cache = ctypes.POINTER(KVCache)
+
 # name -> (restype, argtypes); the single source of the exported symbol list.
 SIGNATURES = {
     "isp_version": (_i, []),
@@ -43,6 +53,13 @@ SIGNATURES = {
     "isp_nvfp4_scales_to_mma": (_i, [_vp, _i64, _i, _vp, _vp]),
     "isp_nvfp4_gemm": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _i, _f, _vp, _vp, _i, _vp, _i, _vp]),
     "isp_nvfp4_gated_up": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _i, _f, _f, _f, _vp, _vp, _vp]),
+    "isp_kv_append": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i, _vp, _i, _cache, _vp]),
+    "isp_kv_gather": (_i, [_cache, _vp, _vp, _i64, _i, _vp, _i, _i64, _i, _vp, _vp, _vp]),
+    "isp_prompt_attention": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64,
+                                  _i64, _f, _i, _vp, _i64, _i64, _vp]),
+    "isp_paged_decode_workspace": (_i, [ctypes.POINTER(_i64)]),
+    "isp_paged_decode": (_i, [_vp, _i, _i64, _i64, _cache, _vp, _i64, _i, _vp, _i, _i, _f, _vp, _i64, _i64, _vp, _i64,
+                              _vp]),
 }
 
 _LIB = None

@@ -4,11 +4,13 @@
 
 #include <mutex>
 
+#include "attention.cuh"
 #include "common.cuh"
 #include "conv.cuh"
 #include "fir.cuh"
 #include "gemm_sm100.cuh"
 #include "decode_sm100.cuh"
+#include "kv_cache.cuh"
 #include "norm_quant.cuh"
 
 namespace isp {
@@ -1021,6 +1023,226 @@ int isp_conv1d_dynamic_noalloc(const void* x, int x_dtype, int64_t B, int C, int
     return st;
   return isp_conv1d(xq, ISP_E4M3, B, C_pad, T, w_packed, CO, KW, stride, dilation, padding, output_padding,
                     transposed, T_out, 0.f, amax, w_scale, bias, y, out_dtype, stream);
+}
+
+}  // extern "C"
+
+// ---- paged key-value cache and attention: validation and dispatch ----
+namespace isp {
+namespace kv {
+
+// Largest heads * tokens style extents a launch covers; every stride product stays in 64 bits.
+constexpr int64_t kMaxTokens = int64_t(1) << 31;
+
+bool cache_type(int t) { return t == ISP_BF16 || t == ISP_F16 || t == ISP_E4M3 || t == ISP_I8; }
+
+int check_cache(const isp_kv_cache_t* c) {
+  if (c == nullptr || c->k == nullptr || c->v == nullptr) return ISP_ERR_ARG;
+  if (!cache_type(c->dtype)) return ISP_ERR_DTYPE;
+  if (is_code(c->dtype) != (c->k_scale != nullptr) || is_code(c->dtype) != (c->v_scale != nullptr)) return ISP_ERR_ARG;
+  if (c->head_dim != 64 && c->head_dim != 128) return ISP_ERR_SHAPE;
+  if (c->pages < 1 || c->page_size < 1 || c->kv_heads < 1 || c->kv_heads > 4096) return ISP_ERR_SHAPE;
+  // row numbers are kept in 32 bits (64-byte rows: more than the card's memory)
+  if (c->pages > 0xFFFFFFFFll / c->kv_heads / c->page_size) return ISP_ERR_SHAPE;
+  if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_scale) || !aligned16(c->v_scale)) return ISP_ERR_ALIGN;
+  return ISP_OK;
+}
+
+int check_table(const int32_t* table, int64_t stride, int width, const int32_t* lengths, int B) {
+  if (table == nullptr || lengths == nullptr) return ISP_ERR_ARG;
+  if (B < 0 || width < 1 || stride < width) return ISP_ERR_SHAPE;
+  return ISP_OK;
+}
+
+// Strides in elements of an operand whose last dimension is contiguous.
+int check_strides(int64_t a, int64_t b, int bytes) {
+  if (a < 0 || b < 0 || a > (int64_t(1) << 40) || b > (int64_t(1) << 40)) return ISP_ERR_SHAPE;
+  return (a * bytes % 16 || b * bytes % 16) ? ISP_ERR_ALIGN : ISP_OK;
+}
+
+Cache cache_of(const isp_kv_cache_t& c) {
+  return Cache{static_cast<uint8_t*>(c.k), static_cast<uint8_t*>(c.v), c.k_scale, c.v_scale, c.pages, c.page_size,
+               c.kv_heads};
+}
+
+// A block takes about 128 rows (K and V of one token: 2 * heads rows).
+int tokens_per_block(int heads) {
+  const int n = 64 / heads;
+  return n < 1 ? 1 : (n > kMaxTokensPerBlock ? kMaxTokensPerBlock : n);
+}
+
+template <int kD, int kIn>
+int append_code(const RowParams& p, int code, unsigned grid, cudaStream_t s) {
+  switch (code) {
+    case ISP_BF16: return launch_pdl(append_kernel<kD, kIn, ISP_BF16>, dim3(grid), dim3(kRowThreads), 0, s, p);
+    case ISP_F16: return launch_pdl(append_kernel<kD, kIn, ISP_F16>, dim3(grid), dim3(kRowThreads), 0, s, p);
+    case ISP_E4M3: return launch_pdl(append_kernel<kD, kIn, ISP_E4M3>, dim3(grid), dim3(kRowThreads), 0, s, p);
+    default: return launch_pdl(append_kernel<kD, kIn, ISP_I8>, dim3(grid), dim3(kRowThreads), 0, s, p);
+  }
+}
+template <int kD>
+int append(const RowParams& p, int in, int code, unsigned grid, cudaStream_t s) {
+  switch (in) {
+    case ISP_BF16: return append_code<kD, ISP_BF16>(p, code, grid, s);
+    case ISP_F16: return append_code<kD, ISP_F16>(p, code, grid, s);
+    default: return append_code<kD, ISP_F32>(p, code, grid, s);
+  }
+}
+template <int kD, int kCode>
+int gather_out(const RowParams& p, int out, unsigned grid, cudaStream_t s) {
+  switch (out) {
+    case ISP_BF16: return launch_pdl(gather_kernel<kD, kCode, ISP_BF16>, dim3(grid), dim3(kRowThreads), 0, s, p);
+    case ISP_F16: return launch_pdl(gather_kernel<kD, kCode, ISP_F16>, dim3(grid), dim3(kRowThreads), 0, s, p);
+    default: return launch_pdl(gather_kernel<kD, kCode, ISP_F32>, dim3(grid), dim3(kRowThreads), 0, s, p);
+  }
+}
+template <int kD>
+int gather(const RowParams& p, int code, int out, unsigned grid, cudaStream_t s) {
+  switch (code) {
+    case ISP_BF16: return gather_out<kD, ISP_BF16>(p, out, grid, s);
+    case ISP_F16: return gather_out<kD, ISP_F16>(p, out, grid, s);
+    case ISP_E4M3: return gather_out<kD, ISP_E4M3>(p, out, grid, s);
+    default: return gather_out<kD, ISP_I8>(p, out, grid, s);
+  }
+}
+
+}  // namespace kv
+
+namespace attn {
+
+bool scale_ok(float s) { return s > 0.f && s <= 3.402823466e38f; }
+
+template <int kD>
+int prompt(const PromptParams& p, int dtype, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((p.q_tokens + kWarps - 1) / kWarps), static_cast<unsigned>(p.heads));
+  return dtype == ISP_BF16 ? launch_pdl(prompt_kernel<kD, ISP_BF16>, grid, dim3(kWarps * 32), 0, s, p)
+                           : launch_pdl(prompt_kernel<kD, ISP_F16>, grid, dim3(kWarps * 32), 0, s, p);
+}
+
+template <int kD, int kType>
+int decode_code(const DecodeParams& p, int code, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(p.heads), static_cast<unsigned>(p.table.batch));
+  switch (code) {
+    case ISP_E4M3: return launch_pdl(decode_kernel<kD, kType, ISP_E4M3>, grid, dim3(kWarps * 32), 0, s, p);
+    case ISP_I8: return launch_pdl(decode_kernel<kD, kType, ISP_I8>, grid, dim3(kWarps * 32), 0, s, p);
+    default: return launch_pdl(decode_kernel<kD, kType, kType>, grid, dim3(kWarps * 32), 0, s, p);
+  }
+}
+template <int kD>
+int decode(const DecodeParams& p, int dtype, int code, cudaStream_t s) {
+  return dtype == ISP_BF16 ? decode_code<kD, ISP_BF16>(p, code, s) : decode_code<kD, ISP_F16>(p, code, s);
+}
+
+}  // namespace attn
+}  // namespace isp
+
+extern "C" {
+
+int isp_kv_append(const void* k, const void* v, int x_dtype, int64_t T, int64_t k_token_stride, int64_t k_head_stride,
+                  int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens, const int32_t* page_table,
+                  int64_t table_stride, int table_width, const int32_t* lengths, int B, const isp_kv_cache_t* cache,
+                  isp_stream_t stream) {
+  using namespace isp::kv;
+  if (k == nullptr || v == nullptr) return ISP_ERR_ARG;
+  if (x_dtype != ISP_BF16 && x_dtype != ISP_F16 && x_dtype != ISP_F32) return ISP_ERR_DTYPE;
+  if (int st = check_cache(cache)) return st;
+  if (int st = check_table(page_table, table_stride, table_width, lengths, B)) return st;
+  if (T < 0 || T >= kMaxTokens || (cu_seqlens == nullptr && T != B)) return ISP_ERR_SHAPE;
+  const int bytes = type_bytes(x_dtype);
+  if (int st = check_strides(k_token_stride, k_head_stride, bytes)) return st;
+  if (int st = check_strides(v_token_stride, v_head_stride, bytes)) return st;
+  if (!isp::aligned16(k) || !isp::aligned16(v)) return ISP_ERR_ALIGN;
+  if (int st = isp::check_device()) return st;
+  if (T == 0 || B == 0) return ISP_OK;
+  RowParams p{cache_of(*cache), {page_table, table_stride, table_width, lengths, B}, cu_seqlens, T,
+              {static_cast<uint8_t*>(const_cast<void*>(k)), static_cast<uint8_t*>(const_cast<void*>(v))},
+              {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, tokens_per_block(cache->kv_heads)};
+  const unsigned grid = static_cast<unsigned>((T + p.tokens_per_block - 1) / p.tokens_per_block);
+  return cache->head_dim == 64 ? append<64>(p, x_dtype, cache->dtype, grid, stream)
+                               : append<128>(p, x_dtype, cache->dtype, grid, stream);
+}
+
+int isp_kv_gather(const isp_kv_cache_t* cache, const int32_t* cu_seqlens, const int32_t* page_table,
+                  int64_t table_stride, int table_width, const int32_t* lengths, int B, int64_t T, int out_dtype,
+                  void* k_out, void* v_out, isp_stream_t stream) {
+  using namespace isp::kv;
+  if (k_out == nullptr || v_out == nullptr) return ISP_ERR_ARG;
+  if (out_dtype != ISP_BF16 && out_dtype != ISP_F16 && out_dtype != ISP_F32) return ISP_ERR_DTYPE;
+  if (int st = check_cache(cache)) return st;
+  if (int st = check_table(page_table, table_stride, table_width, lengths, B)) return st;
+  if (T < 0 || T >= kMaxTokens || (cu_seqlens == nullptr && T != B)) return ISP_ERR_SHAPE;
+  if (!isp::aligned16(k_out) || !isp::aligned16(v_out)) return ISP_ERR_ALIGN;
+  if (int st = isp::check_device()) return st;
+  if (T == 0 || B == 0) return ISP_OK;
+  const int64_t head = cache->head_dim, token = head * cache->kv_heads;
+  RowParams p{cache_of(*cache), {page_table, table_stride, table_width, lengths, B}, cu_seqlens, T,
+              {static_cast<uint8_t*>(k_out), static_cast<uint8_t*>(v_out)}, {token, token}, {head, head},
+              tokens_per_block(cache->kv_heads)};
+  const unsigned grid = static_cast<unsigned>((T + p.tokens_per_block - 1) / p.tokens_per_block);
+  return cache->head_dim == 64 ? gather<64>(p, cache->dtype, out_dtype, grid, stream)
+                               : gather<128>(p, cache->dtype, out_dtype, grid, stream);
+}
+
+int isp_prompt_attention(const void* q, const void* k, const void* v, int dtype, int64_t q_tokens, int64_t k_tokens,
+                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int B, int heads, int kv_heads,
+                         int head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                         int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, float scale, int causal,
+                         void* out, int64_t out_token_stride, int64_t out_head_stride, isp_stream_t stream) {
+  using namespace isp::kv;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || cu_seqlens_q == nullptr || cu_seqlens_k == nullptr)
+    return ISP_ERR_ARG;
+  if (dtype != ISP_BF16 && dtype != ISP_F16) return ISP_ERR_DTYPE;
+  if ((causal != 0 && causal != 1) || !isp::attn::scale_ok(scale)) return ISP_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128) return ISP_ERR_SHAPE;
+  if (heads < 1 || heads > 65535 || kv_heads < 1 || heads % kv_heads != 0) return ISP_ERR_SHAPE;
+  if (B < 0 || q_tokens < 0 || k_tokens < 0 || q_tokens >= kMaxTokens || k_tokens >= kMaxTokens) return ISP_ERR_SHAPE;
+  if (int st = check_strides(q_token_stride, q_head_stride, 2)) return st;
+  if (int st = check_strides(k_token_stride, k_head_stride, 2)) return st;
+  if (int st = check_strides(v_token_stride, v_head_stride, 2)) return st;
+  if (int st = check_strides(out_token_stride, out_head_stride, 2)) return st;
+  if (!isp::aligned16(q) || !isp::aligned16(k) || !isp::aligned16(v) || !isp::aligned16(out)) return ISP_ERR_ALIGN;
+  if (int st = isp::check_device()) return st;
+  if (q_tokens == 0 || B == 0) return ISP_OK;
+  const isp::attn::PromptParams p{
+      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v),
+      static_cast<uint8_t*>(out), q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
+      v_head_stride, out_token_stride, out_head_stride, q_tokens, k_tokens, cu_seqlens_q, cu_seqlens_k, B, heads,
+      kv_heads, scale, causal};
+  return head_dim == 64 ? isp::attn::prompt<64>(p, dtype, stream) : isp::attn::prompt<128>(p, dtype, stream);
+}
+
+int isp_paged_decode_workspace(int64_t* bytes) {
+  if (bytes == nullptr) return ISP_ERR_ARG;
+  *bytes = 256;
+  return ISP_OK;
+}
+
+int isp_paged_decode(const void* q, int dtype, int64_t q_seq_stride, int64_t q_head_stride,
+                     const isp_kv_cache_t* cache, const int32_t* page_table, int64_t table_stride, int table_width,
+                     const int32_t* lengths, int B, int heads, float scale, void* out, int64_t out_seq_stride,
+                     int64_t out_head_stride, void* workspace, int64_t workspace_bytes, isp_stream_t stream) {
+  using namespace isp::kv;
+  if (q == nullptr || out == nullptr || workspace == nullptr) return ISP_ERR_ARG;
+  if (dtype != ISP_BF16 && dtype != ISP_F16) return ISP_ERR_DTYPE;
+  if (int st = check_cache(cache)) return st;
+  if (!is_code(cache->dtype) && cache->dtype != dtype) return ISP_ERR_DTYPE;
+  if (int st = check_table(page_table, table_stride, table_width, lengths, B)) return st;
+  if (!isp::attn::scale_ok(scale)) return ISP_ERR_ARG;
+  if (heads < 1 || heads > 65535 || heads % cache->kv_heads != 0 || B > 65535) return ISP_ERR_SHAPE;
+  if (int st = check_strides(q_seq_stride, q_head_stride, 2)) return st;
+  if (int st = check_strides(out_seq_stride, out_head_stride, 2)) return st;
+  if (!isp::aligned16(q) || !isp::aligned16(out) || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return ISP_ERR_ALIGN;
+  int64_t need = 0;
+  isp_paged_decode_workspace(&need);
+  if (workspace_bytes < need) return ISP_ERR_SHAPE;
+  if (int st = isp::check_device()) return st;
+  if (B == 0) return ISP_OK;
+  const isp::attn::DecodeParams p{cache_of(*cache), {page_table, table_stride, table_width, lengths, B},
+                                  static_cast<const uint8_t*>(q), static_cast<uint8_t*>(out), q_seq_stride,
+                                  q_head_stride, out_seq_stride, out_head_stride, heads, scale};
+  return cache->head_dim == 64 ? isp::attn::decode<64>(p, dtype, cache->dtype, stream)
+                               : isp::attn::decode<128>(p, dtype, cache->dtype, stream);
 }
 
 }  // extern "C"
