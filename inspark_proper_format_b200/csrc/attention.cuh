@@ -21,16 +21,6 @@ struct PromptParams {
   int causal;
 };
 
-struct DecodeParams {
-  kv::Cache cache;
-  kv::Table table;
-  const uint8_t* q;
-  uint8_t* out;
-  int64_t q_seq, q_head, o_seq, o_head;
-  int heads;
-  float scale;
-};
-
 // acc[i] belongs to dim lane * (kD / 32) + i.
 template <int kD>
 struct RowState {
@@ -125,58 +115,6 @@ __global__ void __launch_bounds__(kWarps * 32) prompt_kernel(const PromptParams 
 #pragma unroll
   for (int d = 0; d < kD / 32; ++d)
     store1<kType>(p.out + (i * p.o_token + h * p.o_head + lane * (kD / 32) + d) * kB, st.acc[d] * inv);
-}
-
-// grid (heads, sequences); the block's warps take every kWarps-th step of 32 keys and are joined at the end
-template <int kD, int kType, int kCode>
-__global__ void __launch_bounds__(kWarps * 32) decode_kernel(const DecodeParams p) {
-  constexpr int kB = 2, kC = kv::type_bytes(kCode);
-  __shared__ float qs[kD];
-  __shared__ float ms[kWarps], ls[kWarps], os[kWarps][kD];
-  pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.x, hk = h / (p.heads / p.cache.heads), b = blockIdx.y;
-  if (threadIdx.x < kD) qs[threadIdx.x] = load1<kType>(p.q + (b * p.q_seq + h * p.q_head + threadIdx.x) * kB) * p.scale;
-  __syncthreads();
-  const int64_t len = p.table.lengths[b];
-  RowState<kD> st;
-  for (int64_t j0 = warp * 32; j0 < len; j0 += kWarps * 32) {
-    float s = -INFINITY, vs = 1.f;
-    int64_t row = -1;
-    if (j0 + lane < len) row = kv::row_of(p.cache, p.table, b, j0 + lane);
-    if (row >= 0) {
-      row += static_cast<int64_t>(hk) * p.cache.page_size;
-      s = dot<kD, kCode>(p.cache.k + row * kD * kC, qs);
-      if constexpr (kv::is_code(kCode)) {
-        s *= p.cache.k_scale[row];
-        vs = p.cache.v_scale[row];
-      }
-    }
-    const unsigned mask = __ballot_sync(0xffffffffu, row >= 0);
-    softmax_step<kD>(st, s, mask, [&](int j, int d) {
-      const int64_t r = __shfl_sync(0xffffffffu, row, j);
-      return load1<kCode>(p.cache.v + (r * kD + lane * (kD / 32) + d) * kC) * __shfl_sync(0xffffffffu, vs, j);
-    });
-  }
-  if (lane == 0) {
-    ms[warp] = st.m;
-    ls[warp] = st.l;
-  }
-#pragma unroll
-  for (int d = 0; d < kD / 32; ++d) os[warp][lane * (kD / 32) + d] = st.acc[d];
-  __syncthreads();
-  if (threadIdx.x < kD) {
-    float m = -INFINITY;
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ms[w]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o = 0.f;
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = __expf(ms[w] - base);
-      l += f * ls[w];
-      o += f * os[w][threadIdx.x];
-    }
-    store1<kType>(p.out + (b * p.o_seq + h * p.o_head + threadIdx.x) * kB, l == 0.f ? 0.f : o / l);
-  }
 }
 
 }  // namespace attn

@@ -12,6 +12,7 @@
 #include "decode_sm100.cuh"
 #include "kv_cache.cuh"
 #include "norm_quant.cuh"
+#include "paged_decode.cuh"
 
 namespace isp {
 
@@ -1061,8 +1062,11 @@ int check_strides(int64_t a, int64_t b, int bytes) {
 }
 
 Cache cache_of(const isp_kv_cache_t& c) {
+  int s = 0;
+  while ((1ll << s) < c.page_size) ++s;
+  const uint32_t mul = static_cast<uint32_t>(((1ull << (31 + s)) + c.page_size - 1) / c.page_size);
   return Cache{static_cast<uint8_t*>(c.k), static_cast<uint8_t*>(c.v), c.k_scale, c.v_scale, c.pages, c.page_size,
-               c.kv_heads};
+               c.kv_heads, mul, 31 + s};
 }
 
 // A block takes about 128 rows (K and V of one token: 2 * heads rows).
@@ -1119,18 +1123,44 @@ int prompt(const PromptParams& p, int dtype, cudaStream_t s) {
                            : launch_pdl(prompt_kernel<kD, ISP_F16>, grid, dim3(kWarps * 32), 0, s, p);
 }
 
-template <int kD, int kType>
-int decode_code(const DecodeParams& p, int code, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(p.heads), static_cast<unsigned>(p.table.batch));
-  switch (code) {
-    case ISP_E4M3: return launch_pdl(decode_kernel<kD, kType, ISP_E4M3>, grid, dim3(kWarps * 32), 0, s, p);
-    case ISP_I8: return launch_pdl(decode_kernel<kD, kType, ISP_I8>, grid, dim3(kWarps * 32), 0, s, p);
-    default: return launch_pdl(decode_kernel<kD, kType, kType>, grid, dim3(kWarps * 32), 0, s, p);
+template <int kD, int kCode, int kType>
+int decode(const DecodeParams& p, cudaStream_t s) {
+  using T = Tile<kD, kCode>;
+  auto kern = decode_kernel<kD, kCode, kType>;
+  const int smem = T::smem_bytes(p.gb);
+  // blocks per SM by query heads per key head (the joins and query rows of a block grow with them)
+  static int blocks_per_sm[64][9] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return ISP_ERR_ARCH;
+  if (blocks_per_sm[dev][p.gb] == 0) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::smem_bytes(8)) != cudaSuccess)
+      return ISP_ERR_LAUNCH;
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kDecWarps * 32, smem) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    blocks_per_sm[dev][p.gb] = n;
   }
+  // no more blocks than units of work the page table has room for
+  const int64_t room = static_cast<int64_t>(p.table.width) * p.cache.page_size;
+  const int64_t units = (room + T::kStep - 1) / T::kStep * p.cache.heads * p.gblocks * p.table.batch;
+  int64_t grid = static_cast<int64_t>(blocks_per_sm[dev][p.gb]) * sm_count();
+  if (grid > kMaxBlocks) grid = kMaxBlocks;
+  if (grid > units) grid = units;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kDecWarps * 32), smem, s, p);
 }
+
 template <int kD>
-int decode(const DecodeParams& p, int dtype, int code, cudaStream_t s) {
-  return dtype == ISP_BF16 ? decode_code<kD, ISP_BF16>(p, code, s) : decode_code<kD, ISP_F16>(p, code, s);
+int decode_type(const DecodeParams& p, int dtype, int code, cudaStream_t s) {
+  const bool bf16 = dtype == ISP_BF16;
+  switch (code) {
+    case ISP_E4M3: return bf16 ? decode<kD, ISP_E4M3, ISP_BF16>(p, s) : decode<kD, ISP_E4M3, ISP_F16>(p, s);
+    case ISP_I8: return bf16 ? decode<kD, ISP_I8, ISP_BF16>(p, s) : decode<kD, ISP_I8, ISP_F16>(p, s);
+    case ISP_BF16: return decode<kD, ISP_BF16, ISP_BF16>(p, s);
+    default: return decode<kD, ISP_F16, ISP_F16>(p, s);
+  }
 }
 
 }  // namespace attn
@@ -1213,7 +1243,7 @@ int isp_prompt_attention(const void* q, const void* k, const void* v, int dtype,
 
 int isp_paged_decode_workspace(int64_t* bytes) {
   if (bytes == nullptr) return ISP_ERR_ARG;
-  *bytes = 256;
+  *bytes = isp::attn::kDecWorkspace;
   return ISP_OK;
 }
 
@@ -1238,11 +1268,24 @@ int isp_paged_decode(const void* q, int dtype, int64_t q_seq_stride, int64_t q_h
   if (workspace_bytes < need) return ISP_ERR_SHAPE;
   if (int st = isp::check_device()) return st;
   if (B == 0) return ISP_OK;
-  const isp::attn::DecodeParams p{cache_of(*cache), {page_table, table_stride, table_width, lengths, B},
-                                  static_cast<const uint8_t*>(q), static_cast<uint8_t*>(out), q_seq_stride,
-                                  q_head_stride, out_seq_stride, out_head_stride, heads, scale};
-  return cache->head_dim == 64 ? isp::attn::decode<64>(p, dtype, cache->dtype, stream)
-                               : isp::attn::decode<128>(p, dtype, cache->dtype, stream);
+  isp::attn::DecodeParams p{};
+  p.cache = cache_of(*cache);
+  p.table = {page_table, table_stride, table_width, lengths, B};
+  p.q = static_cast<const uint8_t*>(q);
+  p.out = static_cast<uint8_t*>(out);
+  p.q_seq = q_seq_stride;
+  p.q_head = q_head_stride;
+  p.o_seq = out_seq_stride;
+  p.o_head = out_head_stride;
+  p.heads = heads;
+  p.group = heads / cache->kv_heads;
+  p.gblocks = (p.group + 7) / 8;
+  p.gb = p.group < 8 ? p.group : 8;
+  p.scale = scale * 1.44269504088896340736f;
+  p.counters = static_cast<unsigned*>(workspace);
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + isp::attn::kMaxBlocks * 4);
+  return cache->head_dim == 64 ? isp::attn::decode_type<64>(p, dtype, cache->dtype, stream)
+                               : isp::attn::decode_type<128>(p, dtype, cache->dtype, stream);
 }
 
 }  // extern "C"

@@ -27,7 +27,16 @@ struct Cache {
   int64_t pages;
   int page_size;
   int heads;
+  // n / page_size = (n * page_mul) >> page_shift for 0 <= n < 2^31: page_shift = 31 + s,
+  // 2^s >= page_size, page_mul = ceil(2^page_shift / page_size), whose excess times n stays
+  // below 2^page_shift
+  uint32_t page_mul;
+  int page_shift;
 };
+
+ISP_HD int page_of(const Cache& c, int pos) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(pos)) * c.page_mul) >> c.page_shift);
+}
 
 struct Table {
   const int* pages;      // [batch, stride]
@@ -42,9 +51,9 @@ ISP_D void record_bad_index() { atomicExch(&g_device_error, (int)ISP_ERR_ARG); }
 
 // Row of position `pos` of head 0 of sequence b: (page * heads) * page_size + offset, or
 // -1.  Head h lies h * page_size rows further on.
-ISP_D int64_t row_of(const Cache& c, const Table& t, int b, int64_t pos) {
+ISP_D int64_t row_of(const Cache& c, const Table& t, int b, int pos) {
   if (pos < 0) return -1;
-  const int64_t slot = pos / c.page_size;
+  const int slot = page_of(c, pos);
   if (slot >= t.width) {
     record_bad_index();
     return -1;
@@ -78,7 +87,7 @@ ISP_D int64_t row_of_token(const Cache& c, const Table& t, const int* cu, int64_
     end = cu[b + 1];
     if (i < first || i >= end) return -1;      // a token that no sequence claims
   }
-  return row_of(c, t, b, t.lengths[b] - (end - first) + (i - first));
+  return row_of(c, t, b, static_cast<int>(t.lengths[b] - (end - first) + (i - first)));
 }
 
 // ---- eight elements of a row -------------------------------------------------------------
