@@ -4,7 +4,6 @@
 
 #include <mutex>
 
-#include "attention.cuh"
 #include "common.cuh"
 #include "conv.cuh"
 #include "fir.cuh"
@@ -13,6 +12,7 @@
 #include "kv_cache.cuh"
 #include "norm_quant.cuh"
 #include "paged_decode.cuh"
+#include "prompt_attention.cuh"
 
 namespace isp {
 
@@ -1032,8 +1032,8 @@ int isp_conv1d_dynamic_noalloc(const void* x, int x_dtype, int64_t B, int C, int
 namespace isp {
 namespace kv {
 
-// Largest heads * tokens style extents a launch covers; every stride product stays in 64 bits.
-constexpr int64_t kMaxTokens = int64_t(1) << 31;
+// Tokens of one call; positions and key counts stay in 32 bits, offsets are 64-bit products.
+constexpr int64_t kMaxTokens = int64_t(1) << 30;
 
 bool cache_type(int t) { return t == ISP_BF16 || t == ISP_F16 || t == ISP_E4M3 || t == ISP_I8; }
 
@@ -1116,13 +1116,6 @@ namespace attn {
 
 bool scale_ok(float s) { return s > 0.f && s <= 3.402823466e38f; }
 
-template <int kD>
-int prompt(const PromptParams& p, int dtype, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((p.q_tokens + kWarps - 1) / kWarps), static_cast<unsigned>(p.heads));
-  return dtype == ISP_BF16 ? launch_pdl(prompt_kernel<kD, ISP_BF16>, grid, dim3(kWarps * 32), 0, s, p)
-                           : launch_pdl(prompt_kernel<kD, ISP_F16>, grid, dim3(kWarps * 32), 0, s, p);
-}
-
 template <int kD, int kCode, int kType>
 int decode(const DecodeParams& p, cudaStream_t s) {
   using T = Tile<kD, kCode>;
@@ -1164,6 +1157,47 @@ int decode_type(const DecodeParams& p, int dtype, int code, cudaStream_t s) {
 }
 
 }  // namespace attn
+
+namespace prompt {
+
+// [tokens, heads, head_dim] with element strides as a 3-D map of (64 elements, 1 head, 128 tokens) boxes.
+bool make_rows_map(CUtensorMap* map, const void* base, bool bf16, int head_dim, int heads, int64_t tokens,
+                   int64_t head_stride, int64_t token_stride) {
+  gemm::EncodeFn fn = gemm::encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(token_stride) * 2};
+  cuuint32_t box[3] = {64, 1, kTile};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int kD, bool kBf16>
+int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, cudaStream_t stream) {
+  auto kern = prompt_kernel<kD, kBf16>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return ISP_ERR_ARCH;
+  if (!configured[dev]) {
+    // the roles' register split draws on the registers of the launch: refuse a build that has fewer
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kern) != cudaSuccess || attr.numRegs * kThreads < 2 * 128 * kSoftmaxRegs + 128 * kOtherRegs ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<kD>::kBytes) != cudaSuccess) {
+      cudaGetLastError();
+      return ISP_ERR_LAUNCH;
+    }
+    configured[dev] = true;
+  }
+  // no more blocks than there can be items (the lengths are on the device)
+  const int64_t most = ((p.q_tokens + 2 * kTile - 1) / (2 * kTile) + p.batch) * p.heads;
+  const int64_t grid = most < sm_count() ? most : sm_count();
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Layout<kD>::kBytes, stream, q, k, v, p);
+}
+
+}  // namespace prompt
 }  // namespace isp
 
 extern "C" {
@@ -1230,15 +1264,40 @@ int isp_prompt_attention(const void* q, const void* k, const void* v, int dtype,
   if (int st = check_strides(k_token_stride, k_head_stride, 2)) return st;
   if (int st = check_strides(v_token_stride, v_head_stride, 2)) return st;
   if (int st = check_strides(out_token_stride, out_head_stride, 2)) return st;
+  // rows of a tensor map do not overlap
+  if ((heads > 1 && q_head_stride < head_dim) || (kv_heads > 1 && (k_head_stride < head_dim || v_head_stride < head_dim)) ||
+      (q_tokens > 1 && q_token_stride < head_dim) || (k_tokens > 1 && (k_token_stride < head_dim || v_token_stride < head_dim)))
+    return ISP_ERR_SHAPE;
   if (!isp::aligned16(q) || !isp::aligned16(k) || !isp::aligned16(v) || !isp::aligned16(out)) return ISP_ERR_ALIGN;
   if (int st = isp::check_device()) return st;
   if (q_tokens == 0 || B == 0) return ISP_OK;
-  const isp::attn::PromptParams p{
-      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v),
-      static_cast<uint8_t*>(out), q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
-      v_head_stride, out_token_stride, out_head_stride, q_tokens, k_tokens, cu_seqlens_q, cu_seqlens_k, B, heads,
-      kv_heads, scale, causal};
-  return head_dim == 64 ? isp::attn::prompt<64>(p, dtype, stream) : isp::attn::prompt<128>(p, dtype, stream);
+  if (k_tokens == 0) return ISP_ERR_SHAPE;
+  const bool bf16 = dtype == ISP_BF16;
+  CUtensorMap tq, tk, tv;
+  if (!isp::prompt::make_rows_map(&tq, q, bf16, head_dim, heads, q_tokens, q_head_stride, q_token_stride) ||
+      !isp::prompt::make_rows_map(&tk, k, bf16, head_dim, kv_heads, k_tokens, k_head_stride, k_token_stride) ||
+      !isp::prompt::make_rows_map(&tv, v, bf16, head_dim, kv_heads, k_tokens, v_head_stride, v_token_stride))
+    return ISP_ERR_LAUNCH;
+  isp::prompt::Params p{};
+  p.out = static_cast<uint8_t*>(out);
+  p.v = static_cast<const uint8_t*>(v);
+  p.v_token = v_token_stride;
+  p.v_head = v_head_stride;
+  p.o_token = out_token_stride;
+  p.o_head = out_head_stride;
+  p.q_tokens = q_tokens;
+  p.k_tokens = k_tokens;
+  p.cu_q = cu_seqlens_q;
+  p.cu_k = cu_seqlens_k;
+  p.batch = B;
+  p.heads = heads;
+  p.group = heads / kv_heads;
+  p.scale = scale * 1.44269504088896340736f;
+  p.causal = causal;
+  p.out32 = (reinterpret_cast<uintptr_t>(out) % 32 == 0 && out_token_stride % 16 == 0 && out_head_stride % 16 == 0) ? 1 : 0;
+  if (head_dim == 64)
+    return bf16 ? isp::prompt::launch<64, true>(tq, tk, tv, p, stream) : isp::prompt::launch<64, false>(tq, tk, tv, p, stream);
+  return bf16 ? isp::prompt::launch<128, true>(tq, tk, tv, p, stream) : isp::prompt::launch<128, false>(tq, tk, tv, p, stream);
 }
 
 int isp_paged_decode_workspace(int64_t* bytes) {

@@ -103,10 +103,12 @@ def table_args(page_table: torch.Tensor, lengths: torch.Tensor, device):
 
 def rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [tokens, heads, dim] with strides the kernels take: itself where the last
-    dimension is contiguous and the others are 16-byte multiples, else a copy."""
-    size = t.element_size()
-    if (t.stride(-1) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 and t.stride(0) * size % 16 == 0
-            and t.stride(1) * size % 16 == 0 and t.data_ptr() % 16 == 0):
+    dimension is contiguous and its rows are apart, at multiples of 16 bytes; else a copy."""
+    unit = 16 // t.element_size()
+    tokens, heads, dim = t.shape
+    token, head, last = t.stride()
+    if (last == 1 and token % unit == 0 and head % unit == 0 and t.data_ptr() % 16 == 0
+            and (token >= dim or tokens <= 1) and (head >= dim or heads == 1)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
