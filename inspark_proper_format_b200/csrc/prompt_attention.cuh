@@ -12,16 +12,25 @@
 //                   scores from TMEM, writes p in 16 bits over them, and at the end scales
 //                   and stores the row's output.  m stays up to kSlack behind the maximum,
 //                   so that most steps leave the accumulated output alone.
-//   warp 8          issues the MMAs: S = Q K^T (both operands in shared memory) and
-//                   O += P V (P in TMEM, V's tile read with its keys along K).  For each
-//                   tile PV(j - 1) then S(j), the two tiles in turn, so one tile's softmax
-//                   runs beside the other's MMAs.
+//   warps 8, 11     issue the MMAs of tile 0 and 1: S = Q K^T (both operands in shared memory)
+//                   and O += P V (P in TMEM, V's tile read with its keys along K), PV(j - 1)
+//                   then S(j).  A warp for each tile: the waits of one warp for both were
+//                   the longest chain of the kernel.
 //   warp 9          finds the items and loads Q and the ring of K and V tiles by TMA.
-//   warps 10, 11    check the V tiles that hold keys some row must not see.  A product with
+//   warp 10         checks the V tiles that hold keys some row must not see.  A product with
 //                   p = 0 would turn an infinity or NaN there into NaN, so they are set to
 //                   zero in shared memory; values that other rows do see are added to those
 //                   rows at the end.
 // Every wait is bounded; on expiry the block unwinds as the GEMMs do.
+//
+// Measured on one B200 (power-capped at 1.8 GHz in the long case): 16384 tokens, 32 over 8
+// heads of 128, 2.12 ms (1.04 PFLOP/s of causal work); 64 x 760 frames, 8 heads of 64, every
+// key, 155 us; 64 x 256 tokens, 20 heads of 64, 73 us.  Bound by the softmax: a step of both
+// tiles takes about 3800 cycles, of them 2048 in the special function unit and 1500 in the
+// tensor pipe; what is left is the chain S -> maximum -> exponentials -> PV of a tile.  Tried
+// and slower: half of the exponentials or fewer by polynomial (5 to 25%, the warps are bound by
+// their own instruction chains), a second read of S in a rolled loop (15%), two threads a row
+// (5 to 20% on long items), half of S(j + 1) before PV(j) (4%), no turns (10 to 18%).
 #pragma once
 
 #include "gemm_sm100.cuh"
@@ -46,13 +55,11 @@ struct Params {
 constexpr int kTile = 128;                  // queries of a tile, keys of a step
 constexpr int kThreads = 384;
 constexpr int kItemSlots = 4;
-constexpr int kTmemColumns = 512;           // S0, S1, then O0, O1
+constexpr int kTmemColumns = 512;
 constexpr float kSlack = 8.f;
-#ifndef POLY
-#define POLY 4
-#endif
-constexpr int kPolyEvery = POLY;            // one pair of exponentials in this many goes by polynomial
-// registers of a softmax thread and of the other warps' threads (a sum over the launch's 384 x 168 would wait for ever)
+constexpr int kTurnSteps = 4;               // key tiles from which on the two query tiles take turns
+// Registers of a softmax thread and of the other warps' threads.  They draw on the launch's
+// 384 x 168; a larger sum would wait for ever, so the host checks the build's count.
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
 static_assert(2 * 128 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "");
 
@@ -60,11 +67,14 @@ template <int kD>
 struct Layout {
   static constexpr int kTileBytes = kTile * kD * 2;            // a tile of Q, K or V: kD / 64 boxes of 128 rows x 128 bytes
   static constexpr int kStages = kD == 64 ? 8 : 5;             // K and V tiles in flight
+  static constexpr int kQBuffers = kD == 64 ? 2 : 1;           // blocks of Q: the next item's is loaded early where it fits
   static constexpr int kQ = 0;
-  static constexpr int kRing = 2 * kTileBytes;
+  static constexpr int kRing = kQBuffers * 2 * kTileBytes;
   static constexpr int kBars = kRing + kStages * kTileBytes;
   static constexpr int kBytes = kBars + 1024;
-  static_assert(kStages <= 8, "at most four V tiles in the ring");
+  // TMEM columns of tile t: S, with P over its first half; O
+  static constexpr int s(int t) { return t * kTile; }
+  static constexpr int o(int t) { return 2 * kTile + t * kD; }
 };
 
 struct Item {
@@ -81,7 +91,7 @@ struct Item {
 
 struct Bars {
   uint64_t full[8], empty[8];                        // K and V ring
-  uint64_t q_full, q_free;
+  uint64_t q_full[2], q_free[2];
   uint64_t s_full[2], p_full[2][2], o_full[2], o_free[2];   // p: keys 0-63, then 64-127
   // V tiles through the check, in order: their loads complete on v_in instead of the ring's
   // barrier (which the producer completes by hand), the check answers on v_ok.  The ring
@@ -90,6 +100,7 @@ struct Bars {
   uint64_t item_full[kItemSlots], item_free[kItemSlots];
   uint64_t drained;
   Item items[kItemSlots];
+  uint32_t turn[2];      // steps whose exponentials a tile has taken, times its four warps
   uint32_t tmem;
   int abort;
 };
@@ -155,36 +166,54 @@ ISP_D float max3_nan(float a, float b, float c) {
   return r;
 }
 
-// 2^x for x <= 2^7 without the special function unit: x = n + f with n whole and |f| <= 1/2
-// (adding 1.5 * 2^23 rounds to n), 2^f by the polynomial of least largest relative error on
-// [-1/2, 1/2] (Remez; 2^-13.7 in degree 3, 2^-18.5 in degree 4, below the rounding to BF16
-// and FP16), n added to the exponent.  x below -126 counts as -126.
-template <bool kBf16>
-ISP_D float2 ex2_poly(float2 x) {
-  const float2 magic = make_float2(12582912.f, 12582912.f);
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 r = __fadd2_rn(x, magic);
-  const float2 f = __fadd2_rn(x, __ffma2_rn(r, make_float2(-1.f, -1.f), magic));
-  const auto two = [](float c) { return make_float2(c, c); };
-  float2 y;
-  if constexpr (kBf16) {
-    y = __ffma2_rn(f, two(0.05517167f), two(0.24261113f));
-    y = __ffma2_rn(f, y, two(0.69326097f));
-    y = __ffma2_rn(f, y, two(0.99992806f));
-  } else {
-    y = __ffma2_rn(f, two(0.009570102f), two(0.05591786f));
-    y = __ffma2_rn(f, y, two(0.24024744f));
-    y = __ffma2_rn(f, y, two(0.6931218f));
-    y = __ffma2_rn(f, y, two(0.9999993f));
-  }
-  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(r.x) << 23)),
-                     __int_as_float(__float_as_int(y.y) + (__float_as_int(r.y) << 23)));
+// Bounded wait of a converged warp.  It lies on the chain between the softmax and the MMAs,
+// so the clock is read only after a while (reading it takes longer than most waits).
+ISP_D bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (__all_sync(0xffffffffu, gemm::mbar_try_wait(bar, parity))) return true;
+  return gemm::wait_warp(bar, parity, abort);
+}
+
+// Wait until a count is reached, or for some time: nothing depends on it but the schedule.
+ISP_D void hint_wait(volatile uint32_t* count, uint32_t target) {
+#pragma unroll 1
+  for (int i = 0; i < 128; ++i)
+    if (static_cast<int32_t>(*count - target) >= 0) return;
 }
 
 template <bool kBf16>
 ISP_D uint32_t pack(float a, float b) {
   return kBf16 ? gemm::pack_bf16(a, b) : gemm::pack_f16(a, b);
+}
+
+// ---- 32 of a thread's row of scores ----
+ISP_D void hide(uint32_t (&s)[32], int left) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = i < left ? s[i] : 0xFF800000u;
+}
+ISP_D void take_from(uint32_t (&s)[32], float shift) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - shift);
+}
+ISP_D void chunk_max(const uint32_t (&s)[32], float (&top)[4]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top[e] = max3_nan(top[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
+}
+// 2^(s * scale - base) in 16 bits to TMEM, their sum to l.
+template <bool kBf16>
+ISP_D void chunk_weights(const uint32_t (&s)[32], float scale, float base, float2 (&l)[2], uint32_t taddr) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float a = ex2(fmaf(__uint_as_float(s[2 * i]), scale, -base)), b = ex2(fmaf(__uint_as_float(s[2 * i + 1]), scale, -base));
+    l[i & 1].x += a;
+    l[i & 1].y += b;
+    w[i] = pack<kBf16>(a, b);
+  }
+  tmem_st16(taddr, w);
 }
 
 // Number of 256-query blocks of sequence b (0 where its bounds are bad).
@@ -269,26 +298,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
       gemm::mbar_init(&bars.full[i], 1);
-      gemm::mbar_init(&bars.empty[i], 1);
+      gemm::mbar_init(&bars.empty[i], 2);
     }
-    gemm::mbar_init(&bars.q_full, 1);
-    gemm::mbar_init(&bars.q_free, 1);
     for (int t = 0; t < 2; ++t) {
+      gemm::mbar_init(&bars.q_full[t], 1);
+      gemm::mbar_init(&bars.q_free[t], 2);
       gemm::mbar_init(&bars.s_full[t], 1);
       gemm::mbar_init(&bars.p_full[t][0], 4);
       gemm::mbar_init(&bars.p_full[t][1], 4);
       gemm::mbar_init(&bars.o_full[t], 1);
       gemm::mbar_init(&bars.o_free[t], 4);
+      bars.turn[t] = 0;
     }
     for (int i = 0; i < 4; ++i) {
       gemm::mbar_init(&bars.v_in[i], 1);
-      gemm::mbar_init(&bars.v_ok[i], 2);
+      gemm::mbar_init(&bars.v_ok[i], 1);
     }
     for (int i = 0; i < kItemSlots; ++i) {
       gemm::mbar_init(&bars.item_full[i], 1);
       gemm::mbar_init(&bars.item_free[i], 11);
     }
-    gemm::mbar_init(&bars.drained, 1);
+    gemm::mbar_init(&bars.drained, 2);
     bars.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -334,20 +364,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         if (it.stop) break;
         const int steps = max(it.steps[0], it.steps[1]);
         if (steps == 0) continue;
-        if (loaded > 0 && !(ok = gemm::wait_warp(&bars.q_free, (loaded - 1) & 1, abort))) break;
-        ++loaded;
-        if (lane == 0) {
-          const int tiles = (it.steps[0] > 0) + (it.steps[1] > 0);
-          gemm::mbar_expect_tx(&bars.q_full, tiles * L::kTileBytes);
-          for (int t = 0; t < 2; ++t) {
-            if (it.steps[t] == 0) continue;
-            for (int c = 0; c < kD / 64; ++c)
-              gemm::tma_load_3d(smem + L::kQ + t * L::kTileBytes + c * kTile * 128, &q_map, &bars.q_full, c * 64, it.head,
-                                it.q0 + t * kTile);
+        const auto load_q = [&]() {
+          const int buf = loaded % L::kQBuffers;
+          if (loaded >= L::kQBuffers && !gemm::wait_warp(&bars.q_free[buf], (loaded / L::kQBuffers - 1) & 1, abort)) return false;
+          ++loaded;
+          if (lane == 0) {
+            const int tiles = (it.steps[0] > 0) + (it.steps[1] > 0);
+            gemm::mbar_expect_tx(&bars.q_full[buf], tiles * L::kTileBytes);
+            for (int t = 0; t < 2; ++t) {
+              if (it.steps[t] == 0) continue;
+              for (int c = 0; c < kD / 64; ++c)
+                gemm::tma_load_3d(smem + L::kQ + (buf * 2 + t) * L::kTileBytes + c * kTile * 128, &q_map, &bars.q_full[buf], c * 64,
+                                  it.head, it.q0 + t * kTile);
+            }
           }
-        }
-        __syncwarp();
+          __syncwarp();
+          return true;
+        };
+        // where Q has one buffer, the first K and V go ahead of it: it is free last
+        if (L::kQBuffers == 2 && !(ok = load_q())) break;
         for (int j = 0; j < 2 * steps; ++j, ++kv) {      // K0, V0, K1, V1, ...
+          if (L::kQBuffers == 1 && j == 2 && !(ok = load_q())) break;
           const uint32_t s = kv % L::kStages;
           if (kv >= L::kStages && !(ok = gemm::wait_warp(&bars.empty[s], (kv / L::kStages - 1) & 1, abort))) break;
           const bool check = (j & 1) && (j >> 1) >= it.edge;
@@ -362,96 +399,113 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           edges += check;
           __syncwarp();
         }
+        if (L::kQBuffers == 1 && ok && steps == 1) ok = load_q();
       }
       // loads in flight land before the block ends
       if (*abort) {
-        if (loaded > 0) gemm::wait_warp_drain(&bars.q_full, (loaded - 1) & 1);
+        for (int i = 0; i < L::kQBuffers; ++i)
+          if (loaded > i) gemm::wait_warp_drain(&bars.q_full[i], ((loaded - 1 - i) / L::kQBuffers) & 1);
         for (int i = 0; i < L::kStages; ++i)
           if (kv > static_cast<uint32_t>(i))               // (kv - 1 - i) / kStages: fills of stage i so far, minus one
             gemm::wait_warp_drain(&bars.full[i], ((kv - 1 - i) / L::kStages) & 1);
         for (int i = 0; i < 4; ++i)
           if (edges > static_cast<uint32_t>(i)) gemm::wait_warp_drain(&bars.v_in[i], ((edges - 1 - i) / 4) & 1);
       }
-    } else if (warp == 8) {
-      // ---- MMAs ----
+    } else if (warp != 10) {
+      // ---- MMAs of tile t ----
+      const int t = warp == 8 ? 0 : 1;
       const uint32_t s_desc = idesc(kBf16, kTile, false), o_desc = idesc(kBf16, kD, true);
-      const uint32_t q_addr = gemm::smem_u32(smem + L::kQ), ring = gemm::smem_u32(smem + L::kRing);
-      uint32_t kv = 0;
-      int loaded = 0, edges = 0;
-      int s_count[2] = {0, 0}, o_count[2] = {0, 0};
+      const uint32_t ring = gemm::smem_u32(smem + L::kRing);
+      const uint32_t s_tmem = tmem + L::s(t), o_tmem = tmem + L::o(t);
+      uint64_t q = 0;
+      uint32_t stage = 0, phase = 0;                     // of the ring's next tile
+      uint32_t loaded = 0, edges = 0, count = 0, o_count = 0;
       bool ok = true;
-      for (int64_t n = 0; ok; ++n) {
-        const int slot = static_cast<int>(n % kItemSlots);
-        if (!gemm::wait_warp(&bars.item_full[slot], static_cast<uint32_t>((n / kItemSlots) & 1), abort)) break;
-        const int stop = bars.items[slot].stop, edge = bars.items[slot].edge;
-        const int steps0 = bars.items[slot].steps[0], steps1 = bars.items[slot].steps[1];
+      const auto next = [&]() {
+        if (++stage == L::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      };
+      const auto scores = [&](uint32_t k_stage) {
+        gemm::tc_fence_after();
+        const uint64_t k = gemm::smem_desc_sw128(ring + k_stage * L::kTileBytes);
+#pragma unroll
+        for (int i = 0; i < kD / 16; ++i) {              // 16 head dimensions: 32 bytes of a row
+          const int o = ((i / 4) * kTile * 128 + (i % 4) * 32) >> 4;
+          mma_ss(s_tmem, q + o, k + o, s_desc, i > 0);
+        }
+        gemm::mma_commit_elect<false>(&bars.s_full[t]);
+      };
+      // Give a tile or Q back after the MMAs issued, or at once (the fill was waited for, so the
+      // two warps' arrivals belong to one fill).
+      const auto release = [&](uint64_t* bar, bool used) {
+        if (used) gemm::mma_commit_elect<false>(bar);
+        else if (lane == 0) gemm::mbar_arrive(bar);
+        __syncwarp();
+      };
+      for (uint32_t n = 0; ok; ++n) {
+        const uint32_t slot = n % kItemSlots;
+        if (!wait_all(&bars.item_full[slot], (n / kItemSlots) & 1, abort)) break;
+        const int stop = bars.items[slot].stop, edge = bars.items[slot].edge, mine = bars.items[slot].steps[t];
+        const int steps = max(mine, bars.items[slot].steps[t ^ 1]);
         __syncwarp();
         if (lane == 0) gemm::mbar_arrive(&bars.item_free[slot]);
         if (stop) break;
-        const int steps = max(steps0, steps1);
         if (steps == 0) continue;
-        if (!(ok = gemm::wait_warp(&bars.q_full, loaded & 1, abort))) break;
+        const uint32_t q_buf = loaded % L::kQBuffers;
+        if (!(ok = wait_all(&bars.q_full[q_buf], (loaded / L::kQBuffers) & 1, abort))) break;
         ++loaded;
-        for (int j = 0; j <= steps && ok; ++j) {
-          const uint32_t ik = kv + 2 * j, iv = kv + 2 * j - (j > 0);    // K_j and V_(j - 1) in the ring
-          const uint32_t sk = ik % L::kStages, sv = iv % L::kStages;
-          if (j < steps && !(ok = gemm::wait_warp(&bars.full[sk], (ik / L::kStages) & 1, abort))) break;
-          if (j > 0) {
-            if (j - 1 >= edge) {                                        // checked tiles
-              if (!(ok = gemm::wait_warp(&bars.v_ok[edges & 3], (edges >> 2) & 1, abort))) break;
-              ++edges;
-            } else if (!(ok = gemm::wait_warp(&bars.full[sv], (iv / L::kStages) & 1, abort))) {
-              break;
-            }
+        q = gemm::smem_desc_sw128(gemm::smem_u32(smem + L::kQ) + (q_buf * 2 + t) * L::kTileBytes);
+        if (!(ok = wait_all(&bars.full[stage], phase, abort))) break;
+        if (mine > 0) scores(stage);                     // S(0)
+        release(&bars.empty[stage], mine > 0);
+        if (mine <= 1) release(&bars.q_free[q_buf], mine == 1);
+        next();
+        for (int j = 0; j < steps; ++j) {
+          const uint32_t v_stage = stage, v_phase = phase;             // V_j, then K_(j + 1)
+          next();
+          const uint32_t k_stage = stage;
+          if (j + 1 < steps) {
+            if (!(ok = wait_all(&bars.full[stage], phase, abort))) break;
+            next();
           }
-          gemm::tc_fence_after();
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int mine = t == 0 ? steps0 : steps1;
-            const uint32_t s_tmem = tmem + t * kTile, o_tmem = tmem + 2 * kTile + t * kD;
-            if (j > 0 && j - 1 < mine) {
-              if (j == 1) {
-                if (o_count[t] > 0 && !(ok = gemm::wait_warp(&bars.o_free[t], (o_count[t] - 1) & 1, abort))) break;
-                ++o_count[t];
-              }
-              const uint64_t b = v_desc(ring + sv * L::kTileBytes);
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                if (!(ok = gemm::wait_warp(&bars.p_full[t][half], (s_count[t] - 1) & 1, abort))) break;
-                gemm::tc_fence_after();
-#pragma unroll
-                for (int i = 0; i < kTile / 32; ++i) {                  // 16 keys: 8 columns of P, 2048 bytes of V
-                  const int k = half * (kTile / 32) + i;
-                  mma_ts(o_tmem, s_tmem + k * 8, b + ((k * 2048) >> 4), o_desc, j > 1 || k > 0);
-                }
-              }
-              if (!ok) break;
-              if (j == mine) gemm::mma_commit_elect<false>(&bars.o_full[t]);
-            }
-            if (j < mine) {
-              const uint64_t a = gemm::smem_desc_sw128(q_addr + t * L::kTileBytes);
-              const uint64_t b = gemm::smem_desc_sw128(ring + sk * L::kTileBytes);
-#pragma unroll
-              for (int k = 0; k < kD / 16; ++k) {                       // 16 head dimensions: 32 bytes of a row
-                const int o = ((k / 4) * kTile * 128 + (k % 4) * 32) >> 4;
-                mma_ss(s_tmem, a + o, b + o, s_desc, k > 0);
-              }
-              gemm::mma_commit_elect<false>(&bars.s_full[t]);
-              ++s_count[t];
-            }
+          if (j >= edge) {
+            if (!(ok = wait_all(&bars.v_ok[edges & 3], (edges >> 2) & 1, abort))) break;
+            ++edges;
+          } else if (!(ok = wait_all(&bars.full[v_stage], v_phase, abort))) {
+            break;
           }
-          if (!ok) break;
-          if (j > 0) gemm::mma_commit_elect<false>(&bars.empty[sv]);
-          if (j < steps) gemm::mma_commit_elect<false>(&bars.empty[sk]);
-          if (j == steps - 1) gemm::mma_commit_elect<false>(&bars.q_free);
+          if (j < mine) {
+            if (j == 0 && o_count++ > 0 && !(ok = wait_all(&bars.o_free[t], o_count & 1, abort))) break;
+            const uint64_t v = v_desc(ring + v_stage * L::kTileBytes);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (!(ok = wait_all(&bars.p_full[t][half], count & 1, abort))) break;
+              gemm::tc_fence_after();
+#pragma unroll
+              for (int i = 0; i < kTile / 32; ++i) {     // 16 keys: 8 columns of P, 2048 bytes of V
+                const int k = half * (kTile / 32) + i;
+                mma_ts(o_tmem, s_tmem + k * 8, v + ((k * 2048) >> 4), o_desc, j > 0 || k > 0);
+              }
+            }
+            if (!ok) break;
+            ++count;
+            if (j + 1 == mine) gemm::mma_commit_elect<false>(&bars.o_full[t]);
+            else scores(k_stage);                        // over P, in order behind the products that read it
+          }
+          release(&bars.empty[v_stage], j < mine);
+          if (j + 1 < steps) {
+            release(&bars.empty[k_stage], j + 1 < mine);
+            if (j + 2 == mine) release(&bars.q_free[q_buf], true);
+          }
         }
-        kv += 2 * steps;
       }
       // the MMAs issued end before TMEM is freed
       gemm::mma_commit_elect<false>(&bars.drained);
       gemm::wait_warp_drain(&bars.drained, 0);
     } else {
-      // ---- V check: warps 10 and 11 take 64 keys of a tile each ----
+      // ---- V check ----
       uint32_t kv = 0, edges = 0;
       for (int64_t n = 0;; ++n) {
         const int slot = static_cast<int>(n % kItemSlots);
@@ -463,17 +517,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           const uint32_t i = kv + 2 * j + 1, s = i % L::kStages;
           if (!(ok = gemm::wait_warp(&bars.v_in[edges & 3], (edges >> 2) & 1, abort))) break;
           uint8_t* tile = smem + L::kRing + s * L::kTileBytes;
-          const int first = (warp - 10) * 64;
           uint32_t bad = 0;
-#pragma unroll 4
-          for (int c = 0; c < 64 * kD * 2 / 512; ++c) {                 // 4 rows of 128 bytes a step
-            const uint4 w = *reinterpret_cast<const uint4*>(tile + (c / 16) * kTile * 128 + (first + (c % 16) * 4) * 128 + lane * 16);
+#pragma unroll 8
+          for (int c = 0; c < L::kTileBytes / 512; ++c) {                // 4 rows of 128 bytes a step
+            const uint4 w = *reinterpret_cast<const uint4*>(tile + c * 512 + lane * 16);
             bad |= not_finite<kBf16>(w.x) | not_finite<kBf16>(w.y) | not_finite<kBf16>(w.z) | not_finite<kBf16>(w.w);
           }
           if (__any_sync(0xffffffffu, bad)) {
-            for (int c = 0; c < 64 * kD * 2 / 512; ++c) {
-              const int row = first + (c % 16) * 4 + lane / 8;
-              uint32_t* w = reinterpret_cast<uint32_t*>(tile + (c / 16) * kTile * 128 + (first + (c % 16) * 4) * 128 + lane * 16);
+            for (int c = 0; c < L::kTileBytes / 512; ++c) {
+              const int row = (c % 32) * 4 + lane / 8;
+              uint32_t* w = reinterpret_cast<uint32_t*>(tile + c * 512 + lane * 16);
               for (int e = 0; e < 4; ++e) {
                 if (!not_finite<kBf16>(w[e])) continue;
                 if (j * kTile + row < it.keys) *reinterpret_cast<volatile int*>(&bars.items[slot].flagged) = 1;
@@ -499,53 +552,44 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     // ---- softmax ----
     const int t = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;        // TMEM lane quarter
-    const uint32_t s_tmem = tmem + t * kTile + lanes, o_tmem = tmem + 2 * kTile + t * kD + lanes;
+    const uint32_t s_tmem = tmem + L::s(t) + lanes, o_tmem = tmem + L::o(t) + lanes;
     const int row = t * kTile + (warp & 3) * 32 + lane;                  // row of the block
     const float slack = kSlack / p.scale;
-    int s_count = 0, o_count = 0;
+    uint32_t s_count = 0, o_count = 0, turns = 0;                        // turns: of the other tile, in the items before
     bool ok = true;
-    for (int64_t n = 0; ok; ++n) {
-      const int slot = static_cast<int>(n % kItemSlots);
-      if (!gemm::wait_warp(&bars.item_full[slot], static_cast<uint32_t>((n / kItemSlots) & 1), abort)) break;
-      const Item it = bars.items[slot];
+    for (uint32_t n = 0; ok; ++n) {
+      const uint32_t slot = n % kItemSlots;
+      if (!wait_all(&bars.item_full[slot], (n / kItemSlots) & 1, abort)) break;
+      const Item& it = bars.items[slot];
       if (it.stop) break;
-      const int steps = t == 0 ? it.steps[0] : it.steps[1];
-      const int whole = min(it.keys, max(0, it.off + t * kTile + 1));    // keys that the tile's first row sees
-      const int64_t sees64 = min(static_cast<int64_t>(it.keys), static_cast<int64_t>(it.off) + row + 1);
-      const int sees = static_cast<int>(sees64);                         // keys that this row sees (<= 0: none)
-      float m = -INFINITY;                                               // in units of q.k
+      const int steps = it.steps[t], steps_other = it.steps[t ^ 1];
+      // keys that this row, and the tile's first row, see (<= 0: none)
+      const int sees = static_cast<int>(min(static_cast<int64_t>(it.keys), static_cast<int64_t>(it.off) + row + 1));
+      const int whole = min(it.keys, it.off + t * kTile + 1);
+      const bool take_turns = min(steps, steps_other) >= kTurnSteps;
+      float m = -INFINITY, shift = 0.f, base = 0.f;                      // m in units of q.k
+      bool far = false;
       float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = 0; j < steps; ++j) {
-        if (!(ok = gemm::wait_warp(&bars.s_full[t], s_count & 1, abort))) break;
+        if (!(ok = wait_all(&bars.s_full[t], s_count & 1, abort))) break;
         ++s_count;
         gemm::tc_fence_after();
-        uint32_t raw[kTile / 32][32];
-        float s[kTile];
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         const bool masked = (j + 1) * kTile > whole;
         const int left = sees - j * kTile;                               // keys of this tile that the row sees
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h == 0) {
-            gemm::tmem_ld32(s_tmem, raw[0]);
-            gemm::tmem_ld32(s_tmem + 32, raw[1]);
-            gemm::tmem_ld_wait(raw[0], raw[1]);
-            gemm::tmem_ld32(s_tmem + 64, raw[2]);
-            gemm::tmem_ld32(s_tmem + 96, raw[3]);
-          } else {
-            gemm::tmem_ld_wait(raw[2], raw[3]);
-          }
-#pragma unroll
-          for (int i = h * 64; i < h * 64 + 64; ++i) s[i] = __uint_as_float(raw[i / 32][i % 32]);
-          if (masked) {
-#pragma unroll
-            for (int i = h * 64; i < h * 64 + 64; ++i) s[i] = i < left ? s[i] : -INFINITY;
-          }
-#pragma unroll
-          for (int i = h * 64; i < h * 64 + 64; i += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) tops[e] = max3_nan(tops[e], s[i + 2 * e], s[i + 2 * e + 1]);
-        }
+        uint32_t x[4][32];
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        gemm::tmem_ld32(s_tmem, x[0]);
+        gemm::tmem_ld32(s_tmem + 32, x[1]);
+        gemm::tmem_ld_wait(x[0], x[1]);
+        gemm::tmem_ld32(s_tmem + 64, x[2]);
+        gemm::tmem_ld32(s_tmem + 96, x[3]);
+        if (masked) hide(x[0], left), hide(x[1], left - 32);
+        chunk_max(x[0], tops);
+        chunk_max(x[1], tops);
+        gemm::tmem_ld_wait(x[2], x[3]);
+        if (masked) hide(x[2], left - 64), hide(x[3], left - 96);
+        chunk_max(x[2], tops);
+        chunk_max(x[3], tops);
         const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
         if (__any_sync(0xffffffffu, top > m + slack)) {
           const float now = top > m + slack ? top : m;
@@ -554,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           l[0] = __fmul2_rn(l[0], make_float2(keep, keep));
           l[1] = __fmul2_rn(l[1], make_float2(keep, keep));
           if (j > 0) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < kD / 32; ++c) {
               uint32_t o[32];
               gemm::tmem_ld32(o_tmem + c * 32, o);
@@ -564,47 +608,43 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
               tmem_st32(o_tmem + c * 32, o);
             }
           }
+          // s * scale - m * scale in one rounding; where the second product's own rounding would
+          // count (scores beyond 2^16), the difference is taken first
+          shift = m == -INFINITY ? 0.f : m;
+          far = __any_sync(0xffffffffu, fabsf(shift * p.scale) > 65536.f);
+          base = far ? 0.f : shift * p.scale;
         }
-        // a NaN or an infinite score makes the row NaN (the polynomial below would lose it)
-        if (!(top < INFINITY)) l[0].x = __int_as_float(0x7fc00000);
-        // s * scale - m * scale in one rounding; where the second product's own rounding would
-        // count (scores beyond 2^16), the difference is taken first
-        float base = m == -INFINITY ? 0.f : m * p.scale;
-        if (__any_sync(0xffffffffu, fabsf(base) > 65536.f)) {
-          const float shift = m == -INFINITY ? 0.f : m;
+        if (far) {
 #pragma unroll
-          for (int i = 0; i < kTile; ++i) s[i] -= shift;
-          base = 0.f;
+          for (int c = 0; c < 4; ++c) take_from(x[c], shift);
         }
-        const float2 scale2 = make_float2(p.scale, p.scale), base2 = make_float2(-base, -base);
+        // In long items the tiles take their exponentials in turn, tile 0 of step j, tile 1, tile
+        // 0 of step j + 1: side by side they would share the special function unit and then both
+        // wait for the MMAs.  Only a hint: whoever has waited long goes on.
+        if (take_turns && j > 0)
+          hint_wait(&bars.turn[t ^ 1], 4 * (turns + min(t == 0 ? j : j + 1, steps_other)));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int c = 2 * h; c < 2 * h + 2; ++c) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 x = __ffma2_rn(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), scale2, base2);
-              const float2 e = (i % kPolyEvery) == kPolyEvery - 1 ? ex2_poly<kBf16>(x) : make_float2(ex2(x.x), ex2(x.y));
-              l[i & 1] = __fadd2_rn(l[i & 1], e);
-              w[i] = pack<kBf16>(e.x, e.y);
-            }
-            tmem_st16(s_tmem + c * 16, w);
+        for (int c = 0; c < 4; ++c) {                                    // p replaces the scores
+          chunk_weights<kBf16>(x[c], p.scale, base, l, s_tmem + c * 16);
+          if (c == 2 && lane == 0) atomicAdd(&bars.turn[t], 1u);     // the last quarter may overlap
+          if (c >= 2) {                                                  // half a tile, a chunk later
+            tmem_st_wait();
+            gemm::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) gemm::mbar_arrive(&bars.p_full[t][c - 2]);
           }
-          tmem_st_wait();
-          gemm::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) gemm::mbar_arrive(&bars.p_full[t][h]);
         }
+        if (!(top < INFINITY)) l[0].x = __int_as_float(0x7fc00000);      // a NaN or an infinite score: the row is NaN
       }
       if (!ok) break;
+      turns += steps_other;
       // ---- the row's output ----
       const bool mine = row < it.rows;
       uint8_t* dst = p.out + ((static_cast<int64_t>(it.q0) + row) * p.o_token + it.head * p.o_head) * 2;
       const float sum = (l[0].x + l[0].y) + (l[1].x + l[1].y);
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       if (steps > 0) {
-        if (!(ok = gemm::wait_warp(&bars.o_full[t], o_count & 1, abort))) break;
+        if (!(ok = wait_all(&bars.o_full[t], o_count & 1, abort))) break;
         ++o_count;
         gemm::tc_fence_after();
       }
