@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _lib
-from .kv_cache import PagedKVCache, index_array, rows, table_args
+from .kv_cache import PagedKVCache, call, index_array, rows, table_args
 
 _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -30,7 +30,7 @@ def _softmax_scale(scale, dim):
 
 def _check_out(out, q):
     if out is None:
-        return torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must have the queries' shape, type and device")
     if out.stride(2) != 1 or (out.stride(0) * 2) % 16 or (out.stride(1) * 2) % 16 or out.data_ptr() % 16:
@@ -58,15 +58,16 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     dim, heads, kv_heads = q.shape[2], q.shape[1], k.shape[1]
     if dim not in (64, 128) or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("dim must be 64 or 128 and heads a multiple of kv_heads")
-    index_array(cu_seqlens, "cu_seqlens", q.device)
+    cu = index_array(cu_seqlens, "cu_seqlens", q.device)
     batch = cu_seqlens.shape[0] - 1
     if batch < 0:
         raise ValueError("cu_seqlens holds one more entry than there are sequences")
     if cu_seqlens_k is None:
         if k.shape[0] != q.shape[0]:
             raise ValueError("cu_seqlens_k is needed where queries and keys differ in number")
-        cu_seqlens_k = cu_seqlens
-    index_array(cu_seqlens_k, "cu_seqlens_k", q.device, batch + 1)
+        cu_k = cu
+    else:
+        cu_k = index_array(cu_seqlens_k, "cu_seqlens_k", q.device, batch + 1)
     value = _softmax_scale(scale, dim)
     out = _check_out(out, q)
     if q.shape[0] == 0 or batch == 0:
@@ -74,13 +75,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if k.shape[0] == 0:
         return out.zero_()
     q, k, v = rows(q), rows(k), rows(v)
-    with torch.cuda.device(q.device):
-        status = _lib.load().isp_prompt_attention(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), _TYPES[q.dtype], q.shape[0], k.shape[0], cu_seqlens.data_ptr(),
-            cu_seqlens_k.data_ptr(), batch, heads, kv_heads, dim, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-            v.stride(0), v.stride(1), value, int(bool(causal)), out.data_ptr(), out.stride(0), out.stride(1),
-            _lib.stream_handle(q.device))
-    _lib.check(status, "isp_prompt_attention")
+    call(q.device, "isp_prompt_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), _TYPES[q.dtype], q.shape[0],
+         k.shape[0], cu, cu_k, batch, heads, kv_heads, dim, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], value,
+         int(bool(causal)), out.data_ptr(), *out.stride()[:2])
     return out
 
 
@@ -110,7 +107,7 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: tor
         raise ValueError("q and the cache must be on one CUDA device")
     if q.shape[2] != cache.head_dim or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
         raise ValueError("q does not fit the cache's head_dim and kv_heads")
-    if cache.k_scale is None and cache.k.dtype != q.dtype:
+    if cache.k_scale is None and cache.dtype != q.dtype:
         raise ValueError("a 16-bit cache must have the queries' type")
     table = table_args(page_table, lengths, q.device)
     if table[-1] != q.shape[0]:
@@ -125,11 +122,6 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: tor
     buffer = workspace.buffer
     if buffer.device != q.device:
         raise ValueError("the workspace is on another device")
-    struct = cache.struct()
-    with torch.cuda.device(q.device):
-        status = _lib.load().isp_paged_decode(
-            q.data_ptr(), _TYPES[q.dtype], q.stride(0), q.stride(1), ctypes.byref(struct), *table, q.shape[1], value,
-            out.data_ptr(), out.stride(0), out.stride(1), buffer.data_ptr(), buffer.numel(),
-            _lib.stream_handle(q.device))
-    _lib.check(status, "isp_paged_decode")
+    call(q.device, "isp_paged_decode", q.data_ptr(), _TYPES[q.dtype], *q.stride()[:2], cache.struct, *table, q.shape[1],
+         value, out.data_ptr(), *out.stride()[:2], buffer.data_ptr(), buffer.numel())
     return out

@@ -92,7 +92,7 @@ ISP_D int64_t row_of_token(const Cache& c, const Table& t, const int* cu, int64_
 
 // ---- eight elements of a row -------------------------------------------------------------
 template <int kType>
-ISP_D void load8(const void* p, float (&x)[8]) {
+ISP_D void load8(const void* p, float* x) {
   if constexpr (kType == ISP_F32) {
     const float4 a = *reinterpret_cast<const float4*>(p);
     const float4 b = *(reinterpret_cast<const float4*>(p) + 1);
@@ -100,7 +100,7 @@ ISP_D void load8(const void* p, float (&x)[8]) {
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   } else if constexpr (kType == ISP_BF16) {
     bf16x8_to_f32(*reinterpret_cast<const uint4*>(p), x);
-  } else if constexpr (kType == ISP_F16) {
+  } else {
     const uint4 w = *reinterpret_cast<const uint4*>(p);
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -109,26 +109,18 @@ ISP_D void load8(const void* p, float (&x)[8]) {
       x[2 * i] = f.x;
       x[2 * i + 1] = f.y;
     }
-  } else {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint8_t c = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
-      if constexpr (kType == ISP_E4M3) x[i] = e4m3_to_f32(c);
-      else x[i] = static_cast<float>(static_cast<int8_t>(c));
-    }
   }
 }
 
 template <int kType>
-ISP_D void store8(void* p, const float (&x)[8]) {
+ISP_D void store8(void* p, const float* x) {
   if constexpr (kType == ISP_F32) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
     *(reinterpret_cast<float4*>(p) + 1) = make_float4(x[4], x[5], x[6], x[7]);
   } else if constexpr (kType == ISP_BF16) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16_rn(x[0], x[1]), pack_bf16_rn(x[2], x[3]),
                                               pack_bf16_rn(x[4], x[5]), pack_bf16_rn(x[6], x[7]));
-  } else if constexpr (kType == ISP_F16) {
+  } else {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -136,17 +128,47 @@ ISP_D void store8(void* p, const float (&x)[8]) {
       u[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-  } else {
-    uint32_t u[2] = {0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t c;
-      if constexpr (kType == ISP_E4M3) c = e4m3x2(x[i], 0.f) & 0xFFu;
-      else c = static_cast<uint8_t>(int8_rne_sat(x[i]));
-      u[i / 4] |= c << (8 * (i & 3));
-    }
-    *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
   }
+}
+
+// Sixteen codes.
+template <int kType>
+ISP_D void codes16_to_f32(const uint4& w, float (&x)[16]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kType == ISP_E4M3) {
+      uint32_t a, b;
+      asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+          : "=r"(a), "=r"(b)
+          : "r"(u[i]));
+      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&a)), hi = __half22float2(*reinterpret_cast<const __half2*>(&b));
+      x[4 * i] = lo.x; x[4 * i + 1] = lo.y; x[4 * i + 2] = hi.x; x[4 * i + 3] = hi.y;
+    } else {
+      // 2^23 + (code + 128) as a float, minus 2^23 + 128: exact, and no conversion unit
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[4 * i + j] = __uint_as_float(__byte_perm(u[i] ^ 0x80808080u, 0x4B000000u, 0x7440u + j)) - 8388736.f;
+    }
+  }
+}
+template <int kType>
+ISP_D uint4 f32_to_codes16(const float (&x)[16]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kType == ISP_E4M3) {
+      u[i] = static_cast<uint32_t>(e4m3x2(x[4 * i], x[4 * i + 1])) | (static_cast<uint32_t>(e4m3x2(x[4 * i + 2], x[4 * i + 3])) << 16);
+    } else {
+      // |x| <= 127 after rounding: adding 1.5 * 2^23 rounds to the nearest even integer, whose low
+      // byte is the code
+      uint32_t b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(__fadd_rn(x[4 * i + j], 12582912.f));
+      u[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    }
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
 ISP_HD constexpr int type_bytes(int t) { return t == ISP_F32 ? 4 : (t == ISP_BF16 || t == ISP_F16 ? 2 : 1); }
@@ -164,47 +186,104 @@ struct RowParams {
 
 constexpr int kRowThreads = 256;
 constexpr int kMaxTokensPerBlock = 64;
+constexpr int kBoundsAtOnce = 1024;            // sequences whose bounds a block keeps in shared memory
 
-// kD / 8 lanes hold one row; a block covers tokens_per_block tokens x all heads x {K, V}.
+// Rows (head 0) of the block's tokens into `rows`; returns their number.  A search in global
+// memory is a chain of dependent loads, so the bounds are copied first where they fit.
+ISP_D int find_rows(const RowParams& p, int64_t first, int64_t (&rows)[kMaxTokensPerBlock], int (&bounds)[kBoundsAtOnce + 1]) {
+  const int n = static_cast<int>(min(static_cast<int64_t>(p.tokens_per_block), p.tokens - first));
+  const int* cu = p.cu;
+  if (cu != nullptr && p.table.batch <= kBoundsAtOnce) {
+    for (int i = threadIdx.x; i <= p.table.batch; i += kRowThreads) bounds[i] = p.cu[i];
+    __syncthreads();
+    cu = bounds;
+  }
+  if (threadIdx.x < n) rows[threadIdx.x] = row_of_token(p.cache, p.table, cu, first + threadIdx.x);
+  __syncthreads();
+  return n;
+}
+
+// The rows of a block, a group's every `by`-th: number i is token i % n of head i / n % heads of
+// K or V, so neighbouring groups read and write neighbouring rows of a page.
+struct RowWalk {
+  int token, head, kv, n, heads, d_token, d_head, d_kv;
+  ISP_D RowWalk(int first, int by, int n_, int heads_) : n(n_), heads(heads_) {
+    token = first % n;
+    head = first / n % heads;
+    kv = first / n / heads;
+    d_token = by % n;
+    d_head = by / n % heads;
+    d_kv = by / n / heads;
+  }
+  ISP_D bool inside() const { return kv < 2; }
+  ISP_D void advance() {
+    token += d_token;
+    head += d_head;
+    kv += d_kv;
+    if (token >= n) {
+      token -= n;
+      ++head;
+    }
+    if (head >= heads) {
+      head -= heads;
+      ++kv;
+    }
+  }
+};
+
+// Both kernels are bound by the bytes they move: 16 elements a lane (8 for 16-bit caches),
+// kD / 16 lanes a row, blocks of 256 rows or so (fewer where the call has few tokens), so that
+// the look-up of a block's tokens is a small part of it (64 rows 1 to 50% slower, 1024 rows
+// 30%).  One row a lane at a time: two or four in flight cost registers, and with them more
+// than they hid (10 and 45%).  Measured, append then gather on one B200: INT8, 64 x 256
+// tokens, 20 heads of 64, 65 us (4.0 TB/s of 257 MB); E4M3, 44246 tokens, 8 heads of 128,
+// 115 us (4.8 TB/s of 549 MB).
 template <int kD, int kIn, int kCode>
 __global__ void __launch_bounds__(kRowThreads) append_kernel(const RowParams p) {
-  constexpr int kLanes = kD / 8;
+  constexpr int kElems = is_code(kCode) ? 16 : 8, kLanes = kD / kElems;
   __shared__ int64_t rows[kMaxTokensPerBlock];
+  __shared__ int bounds[kBoundsAtOnce + 1];
   pdl_wait();
+  pdl_trigger();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block;
-  const int n = static_cast<int>(min(static_cast<int64_t>(p.tokens_per_block), p.tokens - first));
-  if (threadIdx.x < n) rows[threadIdx.x] = row_of_token(p.cache, p.table, p.cu, first + threadIdx.x);
-  __syncthreads();
+  const int n = find_rows(p, first, rows, bounds);
   const int lane = threadIdx.x % kLanes;
-  const int per_token = 2 * p.cache.heads;
-  for (int i = threadIdx.x / kLanes; i < n * per_token; i += kRowThreads / kLanes) {
-    const int tok = i / per_token;
-    const int kv = (i % per_token) / p.cache.heads, h = i % p.cache.heads;
-    const int64_t row0 = rows[tok];
-    if (row0 < 0) continue;                     // uniform over the row's lanes
-    float x[8];
-    load8<kIn>(p.x[kv] + ((first + tok) * p.token_stride[kv] + h * p.head_stride[kv] + lane * 8) * type_bytes(kIn), x);
-    const int64_t row = row0 + static_cast<int64_t>(h) * p.cache.page_size;
-    uint8_t* dst = (kv ? p.cache.v : p.cache.k) + (row * kD + lane * 8) * type_bytes(kCode);
-    if constexpr (is_code(kCode)) {
-      float amax = 0.f;
-      bool finite = true;
+  RowWalk at(threadIdx.x / kLanes, kRowThreads / kLanes, n, p.cache.heads);
+  for (; __any_sync(0xffffffffu, at.inside()); at.advance()) {
+    float x[kElems];
+    int64_t row = at.inside() ? rows[at.token] : -1;
+    if (row >= 0) {
+      row += static_cast<int64_t>(at.head) * p.cache.page_size;
+      const uint8_t* src = p.x[at.kv] + ((first + at.token) * p.token_stride[at.kv] + at.head * p.head_stride[at.kv] + lane * kElems) * type_bytes(kIn);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        amax = fmaxf(amax, fabsf(x[j]));
-        finite = finite && (fabsf(x[j]) < __int_as_float(0x7f800000));
-      }
-      if (!finite) amax = __int_as_float(0x7f800000);
-      const unsigned mask = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u)) << ((threadIdx.x & 31) / kLanes * kLanes);
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
-      const bool ok = amax < __int_as_float(0x7f800000);
-      const float s = fmaxf(__fdiv_rn(amax, kCode == ISP_E4M3 ? 448.f : 127.f), 1e-12f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = ok ? __fdiv_rn(x[j], s) : 0.f;
-      store8<kCode>(dst, x);
-      if (lane == 0) (kv ? p.cache.v_scale : p.cache.k_scale)[row] = ok ? s : __int_as_float(0x7fc00000);
+      for (int e = 0; e < kElems; e += 8) load8<kIn>(src + e * type_bytes(kIn), &x[e]);
     } else {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) x[e] = 0.f;
+    }
+    uint8_t* dst = (at.kv == 0 ? p.cache.k : p.cache.v) + (row * kD + lane * kElems) * type_bytes(kCode);
+    if constexpr (is_code(kCode)) {
+      // the largest magnitude as bits, which also order infinities and NaN above the rest
+      uint32_t top = 0u;
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const bool ok = top < 0x7F800000u;
+      const float s = fmaxf(__fdiv_rn(__uint_as_float(top), kCode == ISP_E4M3 ? 448.f : 127.f), 1e-12f);
+      const float y = __fdiv_rn(1.f, s);
+      // RN(x / s) as in div_rn_recip; |x / s| <= 448 (1 + 2^-22) and 1e-12 <= s < 2^122, so its
+      // range checks never apply
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        const float q = __fmul_rn(x[e], y);
+        x[e] = ok ? __fmaf_rn(__fmaf_rn(-q, s, x[e]), y, q) : 0.f;
+      }
+      if (row >= 0) {
+        *reinterpret_cast<uint4*>(dst) = f32_to_codes16<kCode>(x);
+        if (lane == 0) (at.kv == 0 ? p.cache.k_scale : p.cache.v_scale)[row] = ok ? s : __int_as_float(0x7fc00000);
+      }
+    } else if (row >= 0) {
       store8<kCode>(dst, x);
     }
   }
@@ -212,30 +291,35 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(const RowParams p) 
 
 template <int kD, int kCode, int kOut>
 __global__ void __launch_bounds__(kRowThreads) gather_kernel(const RowParams p) {
-  constexpr int kLanes = kD / 8;
+  constexpr int kElems = is_code(kCode) ? 16 : 8, kLanes = kD / kElems;
   __shared__ int64_t rows[kMaxTokensPerBlock];
+  __shared__ int bounds[kBoundsAtOnce + 1];
   pdl_wait();
+  pdl_trigger();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block;
-  const int n = static_cast<int>(min(static_cast<int64_t>(p.tokens_per_block), p.tokens - first));
-  if (threadIdx.x < n) rows[threadIdx.x] = row_of_token(p.cache, p.table, p.cu, first + threadIdx.x);
-  __syncthreads();
+  const int n = find_rows(p, first, rows, bounds);
   const int lane = threadIdx.x % kLanes;
-  const int per_token = 2 * p.cache.heads;
-  for (int i = threadIdx.x / kLanes; i < n * per_token; i += kRowThreads / kLanes) {
-    const int tok = i / per_token;
-    const int kv = (i % per_token) / p.cache.heads, h = i % p.cache.heads;
-    const int64_t row0 = rows[tok];
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (row0 >= 0) {
-      const int64_t row = row0 + static_cast<int64_t>(h) * p.cache.page_size;
-      load8<kCode>((kv ? p.cache.v : p.cache.k) + (row * kD + lane * 8) * type_bytes(kCode), x);
-      if constexpr (is_code(kCode)) {
-        const float s = (kv ? p.cache.v_scale : p.cache.k_scale)[row];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], s);
-      }
+  RowWalk at(threadIdx.x / kLanes, kRowThreads / kLanes, n, p.cache.heads);
+  for (; at.inside(); at.advance()) {
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    float scale = 0.f;
+    int64_t row = rows[at.token];
+    if (row >= 0) {
+      row += static_cast<int64_t>(at.head) * p.cache.page_size;
+      w = *reinterpret_cast<const uint4*>((at.kv == 0 ? p.cache.k : p.cache.v) + (row * kD + lane * kElems) * type_bytes(kCode));
+      if constexpr (is_code(kCode)) scale = (at.kv == 0 ? p.cache.k_scale : p.cache.v_scale)[row];
     }
-    store8<kOut>(p.x[kv] + ((first + tok) * p.token_stride[kv] + h * p.head_stride[kv] + lane * 8) * type_bytes(kOut), x);
+    float x[kElems];
+    if constexpr (is_code(kCode)) {
+      codes16_to_f32<kCode>(w, x);
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) x[e] = __fmul_rn(x[e], scale);
+    } else {
+      load8<kCode>(&w, x);
+    }
+    uint8_t* dst = p.x[at.kv] + ((first + at.token) * p.token_stride[at.kv] + at.head * p.head_stride[at.kv] + lane * kElems) * type_bytes(kOut);
+#pragma unroll
+    for (int e = 0; e < kElems; e += 8) store8<kOut>(dst + e * type_bytes(kOut), x + e);
   }
 }
 

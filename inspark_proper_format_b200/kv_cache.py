@@ -28,6 +28,9 @@ FORMATS = {"bf16": torch.bfloat16, "f16": torch.float16, "e4m3": torch.float8_e4
 _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32,
           torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.I8}
 
+# the current stream's handle without the Python stream object (2 us of a 15 us call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
 
 class PagedKVCache:
     """K and V pools [pages, kv_heads, page_size, head_dim], with FP32 scales
@@ -74,31 +77,46 @@ class PagedKVCache:
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.fmt = next(name for name, dtype in FORMATS.items() if dtype == k.dtype)
         self.device = k.device
+        self.dtype = k.dtype
+        self._struct = _lib.KVCache(_lib.ptr(k), _lib.ptr(v), _lib.ptr(k_scale), _lib.ptr(v_scale), self.pages,
+                                    _TYPES[k.dtype], self.page_size, self.kv_heads, self.head_dim)
+        self.struct = ctypes.byref(self._struct)          # the C ABI's description of this cache
 
-    def struct(self) -> _lib.KVCache:
-        """The C ABI's description of this cache."""
-        return _lib.KVCache(_lib.ptr(self.k), _lib.ptr(self.v), _lib.ptr(self.k_scale), _lib.ptr(self.v_scale),
-                            self.pages, _TYPES[self.k.dtype], self.page_size, self.kv_heads, self.head_dim)
 
-
-def index_array(t: torch.Tensor, name: str, device, shape=None) -> torch.Tensor:
-    """Check an int32 CUDA index array of the given shape (contiguous, 1-D)."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_cuda or t.device != device:
+def index_array(t: torch.Tensor, name: str, device, size=None) -> int:
+    """The pointer of an int32 CUDA index array (1-D, contiguous, of ``size`` elements)."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or not t.is_cuda or t.device != device:
         raise ValueError(f"{name} must be an int32 CUDA tensor on the operands' device")
-    if t.ndim != 1 or not t.is_contiguous() or (shape is not None and t.shape[0] != shape):
-        raise ValueError(f"{name} must be contiguous with {shape if shape is not None else 'its'} elements")
-    return t
+    shape = t.shape
+    if len(shape) != 1 or (size is not None and shape[0] != size) or (t.stride(0) != 1 and shape[0] > 1):
+        raise ValueError(f"{name} must be contiguous with {size if size is not None else 'its'} elements")
+    return t.data_ptr()
 
 
 def table_args(page_table: torch.Tensor, lengths: torch.Tensor, device):
     """(pointer, row stride, width, lengths pointer, batch) of a page table and its lengths."""
-    if (not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or not page_table.is_cuda
-            or page_table.device != device or page_table.ndim != 2 or page_table.shape[1] < 1
-            or page_table.stride(1) != 1):
+    if (not isinstance(page_table, torch.Tensor) or page_table.dtype is not torch.int32 or not page_table.is_cuda
+            or page_table.device != device or page_table.ndim != 2):
         raise ValueError("page_table must be an int32 CUDA tensor [batch, pages per sequence]")
     batch, width = page_table.shape
-    index_array(lengths, "lengths", device, batch)
-    return page_table.data_ptr(), max(page_table.stride(0), width), width, lengths.data_ptr(), batch
+    stride, last = page_table.stride()
+    if width < 1 or (last != 1 and width > 1):
+        raise ValueError("page_table must be an int32 CUDA tensor [batch, pages per sequence]")
+    return page_table.data_ptr(), max(stride, width), width, index_array(lengths, "lengths", device, batch), batch
+
+
+def call(device, name: str, *args) -> None:
+    """Run a C entry point on the device's current stream (its last argument) and raise on an
+    error status.  The current device is switched only where it is another one."""
+    fn = getattr(_lib.load(), name)
+    stream = _raw_stream(device.index) if _raw_stream is not None else _lib.stream_handle(device)
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, stream)
+    if status:
+        _lib.check(status, name)
 
 
 def rows(t: torch.Tensor) -> torch.Tensor:
@@ -125,21 +143,16 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_table:
     if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError("k and v must both be BF16, FP16 or FP32")
     table = table_args(page_table, lengths, cache.device)
-    batch = table[-1]
-    if cu_seqlens is None:
-        if k.shape[0] != batch:
-            raise ValueError("without cu_seqlens there is one token per sequence")
-    else:
-        index_array(cu_seqlens, "cu_seqlens", cache.device, batch + 1)
+    cu = None
+    if cu_seqlens is not None:
+        cu = index_array(cu_seqlens, "cu_seqlens", cache.device, table[-1] + 1)
+    elif k.shape[0] != table[-1]:
+        raise ValueError("without cu_seqlens there is one token per sequence")
     if k.shape[0] == 0:
         return
     k, v = rows(k), rows(v)
-    struct = cache.struct()
-    with torch.cuda.device(cache.device):
-        status = _lib.load().isp_kv_append(
-            k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k.shape[0], k.stride(0), k.stride(1), v.stride(0),
-            v.stride(1), _lib.ptr(cu_seqlens), *table, ctypes.byref(struct), _lib.stream_handle(cache.device))
-    _lib.check(status, "isp_kv_append")
+    call(cache.device, "isp_kv_append", k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k.shape[0], k.stride(0),
+         k.stride(1), v.stride(0), v.stride(1), cu, *table, cache.struct)
 
 
 def kv_gather(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -153,21 +166,17 @@ def kv_gather(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tens
         raise ValueError("rows are read back as BF16, FP16 or FP32")
     table = table_args(page_table, lengths, cache.device)
     batch = table[-1]
+    cu = None
     if cu_seqlens is None:
         if tokens not in (None, batch):
             raise ValueError("without cu_seqlens there is one token per sequence")
         tokens = batch
     else:
-        index_array(cu_seqlens, "cu_seqlens", cache.device, batch + 1)
+        cu = index_array(cu_seqlens, "cu_seqlens", cache.device, batch + 1)
         if tokens is None or tokens < 0:
             raise ValueError("tokens must give the number of packed rows")
     make = torch.empty if batch else torch.zeros
-    out = [make(tokens, cache.kv_heads, cache.head_dim, device=cache.device, dtype=dtype) for _ in range(2)]
-    if tokens == 0:
-        return out[0], out[1]
-    struct = cache.struct()
-    with torch.cuda.device(cache.device):
-        status = _lib.load().isp_kv_gather(ctypes.byref(struct), _lib.ptr(cu_seqlens), *table, tokens, _TYPES[dtype],
-                                           out[0].data_ptr(), out[1].data_ptr(), _lib.stream_handle(cache.device))
-    _lib.check(status, "isp_kv_gather")
-    return out[0], out[1]
+    k, v = make((2, tokens, cache.kv_heads, cache.head_dim), device=cache.device, dtype=dtype).unbind(0)
+    if tokens and batch:
+        call(cache.device, "isp_kv_gather", cache.struct, cu, *table, tokens, _TYPES[dtype], k.data_ptr(), v.data_ptr())
+    return k, v
