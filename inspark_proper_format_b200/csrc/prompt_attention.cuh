@@ -24,13 +24,16 @@
 // Every wait is bounded; on expiry the block unwinds as the GEMMs do.
 //
 // Measured on one B200 (power-capped at 1.8 GHz in the long case): 16384 tokens, 32 over 8
-// heads of 128, 2.12 ms (1.04 PFLOP/s of causal work); 64 x 760 frames, 8 heads of 64, every
-// key, 155 us; 64 x 256 tokens, 20 heads of 64, 73 us.  Bound by the softmax: a step of both
-// tiles takes about 3800 cycles, of them 2048 in the special function unit and 1500 in the
+// heads of 128, 2.01 ms (1.09 PFLOP/s of causal work); 64 x 760 frames, 8 heads of 64, every
+// key, 139 us; 64 x 256 tokens, 20 heads of 64, 60.5 us.  Bound by the softmax: a step of both
+// tiles takes about 3700 cycles, of them 2048 in the special function unit and 1500 in the
 // tensor pipe; what is left is the chain S -> maximum -> exponentials -> PV of a tile.  Tried
 // and slower: half of the exponentials or fewer by polynomial (5 to 25%, the warps are bound by
 // their own instruction chains), a second read of S in a rolled loop (15%), two threads a row
-// (5 to 20% on long items), half of S(j + 1) before PV(j) (4%), no turns (10 to 18%).
+// (5 to 20% on long items), half of S(j + 1) before PV(j) (4%), no turns (10 to 18%).  The
+// roles' code has to stay small, they share the instruction cache: rolling the output and the
+// repair of non-finite values alone took 3 to 8% off, two scores to an instruction (f32x2) in
+// the products and sums of the exponentials another 3 to 9%.
 #pragma once
 
 #include "gemm_sm100.cuh"
@@ -189,12 +192,17 @@ ISP_D uint32_t pack(float a, float b) {
 
 // ---- 32 of a thread's row of scores ----
 ISP_D void hide(uint32_t (&s)[32], int left) {
+  const uint32_t seen = left >= 32 ? 0xFFFFFFFFu : (1u << max(left, 0)) - 1u;   // bits turn into predicates in groups
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i] = i < left ? s[i] : 0xFF800000u;
+  for (int i = 0; i < 32; ++i) s[i] = (seen >> i) & 1u ? s[i] : 0xFF800000u;
 }
 ISP_D void take_from(uint32_t (&s)[32], float shift) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - shift);
+  for (int i = 0; i < 32; i += 2) {
+    const float2 d = __fadd2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(-shift, -shift));
+    s[i] = __float_as_uint(d.x);
+    s[i + 1] = __float_as_uint(d.y);
+  }
 }
 ISP_D void chunk_max(const uint32_t (&s)[32], float (&top)[4]) {
 #pragma unroll
@@ -208,12 +216,17 @@ ISP_D void chunk_weights(const uint32_t (&s)[32], float scale, float base, float
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float a = ex2(fmaf(__uint_as_float(s[2 * i]), scale, -base)), b = ex2(fmaf(__uint_as_float(s[2 * i + 1]), scale, -base));
-    l[i & 1].x += a;
-    l[i & 1].y += b;
+    const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), make_float2(scale, scale), make_float2(-base, -base));
+    const float a = ex2(x.x), b = ex2(x.y);
+    l[i & 1] = __fadd2_rn(l[i & 1], make_float2(a, b));
     w[i] = pack<kBf16>(a, b);
   }
   tmem_st16(taddr, w);
+}
+
+template <bool kBf16>
+ISP_D float to_float(uint16_t bits) {
+  return kBf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
 }
 
 // Number of 256-query blocks of sequence b (0 where its bounds are bad).
@@ -648,53 +661,51 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         ++o_count;
         gemm::tc_fence_after();
       }
-      const bool flagged = steps > 0 && *reinterpret_cast<volatile int*>(&bars.items[slot].flagged) != 0;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < kD / 32; ++c) {
         uint32_t o[32];
         if (steps > 0) {
           gemm::tmem_ld32(o_tmem + c * 32, o);
           gemm::tmem_ld_wait(o);
+          if (c == kD / 32 - 1) {
+            gemm::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) gemm::mbar_arrive(&bars.o_free[t]);
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (c == kD / 32 - 1 && steps > 0) {
-          gemm::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) gemm::mbar_arrive(&bars.o_free[t]);
+        if (!mine) continue;
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = pack<kBf16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+        if (p.out32) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c * 64 + i * 32),
+                         "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]), "r"(w[8 * i + 4]),
+                         "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
+                         : "memory");
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(dst + c * 64 + i * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         }
-        float f[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * inv;
-        if (flagged && mine) {                           // what the V check set to zero and this row sees
-          for (int k = it.edge * kTile; k < sees; ++k) {
-            const uint8_t* v = p.v + ((static_cast<int64_t>(it.k0) + k) * p.v_token + (it.head / p.group) * p.v_head + c * 32) * 2;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const uint32_t bits = *reinterpret_cast<const uint16_t*>(v + i * 2);
-              if (not_finite<kBf16>(bits))
-                f[i] += kBf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(bits)));
-            }
+      }
+      if (steps > 0 && mine && *reinterpret_cast<const volatile int*>(&it.flagged) != 0) {
+        // what the V check set to zero and this row sees: infinities and NaN, which take the element over
+        const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + (it.head / p.group) * p.v_head;
+        uint16_t* out = reinterpret_cast<uint16_t*>(dst);
+#pragma unroll 1
+        for (int k = it.edge * kTile; k < sees; ++k)
+#pragma unroll 1
+          for (int i = 0; i < kD; ++i) {
+            const uint16_t bits = v[(static_cast<int64_t>(it.k0) + k) * p.v_token + i];
+            if (!not_finite<kBf16>(bits)) continue;
+            const uint32_t sum = pack<kBf16>(to_float<kBf16>(out[i]) + to_float<kBf16>(bits), 0.f);
+            out[i] = static_cast<uint16_t>(sum);
           }
-        }
-        if (mine) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = pack<kBf16>(f[2 * i], f[2 * i + 1]);
-          if (p.out32) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c * 64 + i * 32),
-                           "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]), "r"(w[8 * i + 4]),
-                           "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
-                           : "memory");
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<uint4*>(dst + c * 64 + i * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-          }
-        }
       }
       __syncwarp();
       if (lane == 0) gemm::mbar_arrive(&bars.item_free[slot]);
