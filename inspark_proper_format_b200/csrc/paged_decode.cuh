@@ -303,8 +303,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
   at.b = first[0];
   at.len = first[1];
   at.steps = (at.len + kStep - 1) / kStep;
-  at.hg = static_cast<int>(u0 - line[1]) / at.steps;
-  at.step = static_cast<int>(u0 - line[1]) - at.hg * at.steps;
+  at.hg = static_cast<int>((u0 - line[1]) / at.steps);
+  at.step = static_cast<int>((u0 - line[1]) % at.steps);
   Cursor ahead = at;                                   // the unit whose copies start next
   int issued = 0;
 
