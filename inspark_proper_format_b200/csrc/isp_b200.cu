@@ -1169,7 +1169,9 @@ bool make_rows_map(CUtensorMap* map, const void* base, bool bf16, int head_dim, 
   gemm::EncodeFn fn = gemm::encode_fn();
   if (fn == nullptr) return false;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(token_stride) * 2};
+  // the stride of a dimension of one element can be anything
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? head_stride : head_dim) * 2,
+                           static_cast<cuuint64_t>(tokens > 1 ? token_stride : head_dim) * 2};
   cuuint32_t box[3] = {64, 1, kTile};
   cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
@@ -1262,14 +1264,15 @@ int isp_prompt_attention(const void* q, const void* k, const void* v, int dtype,
   if ((causal != 0 && causal != 1) || !isp::attn::scale_ok(scale)) return ISP_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return ISP_ERR_SHAPE;
   if (heads < 1 || heads > 65535 || kv_heads < 1 || heads % kv_heads != 0) return ISP_ERR_SHAPE;
-  if (B < 0 || q_tokens < 0 || k_tokens < 0 || q_tokens >= kMaxTokens || k_tokens >= kMaxTokens) return ISP_ERR_SHAPE;
+  if (B < 0 || B > 65536 || q_tokens < 0 || k_tokens < 0 || q_tokens >= kMaxTokens || k_tokens >= kMaxTokens) return ISP_ERR_SHAPE;
   if (int st = check_strides(q_token_stride, q_head_stride, 2)) return st;
   if (int st = check_strides(k_token_stride, k_head_stride, 2)) return st;
   if (int st = check_strides(v_token_stride, v_head_stride, 2)) return st;
   if (int st = check_strides(out_token_stride, out_head_stride, 2)) return st;
-  // rows of a tensor map do not overlap
+  // rows of a tensor map, and those of the output, do not overlap
   if ((heads > 1 && q_head_stride < head_dim) || (kv_heads > 1 && (k_head_stride < head_dim || v_head_stride < head_dim)) ||
-      (q_tokens > 1 && q_token_stride < head_dim) || (k_tokens > 1 && (k_token_stride < head_dim || v_token_stride < head_dim)))
+      (k_tokens > 1 && (k_token_stride < head_dim || v_token_stride < head_dim)) ||
+      (q_tokens > 1 && (q_token_stride < head_dim || out_token_stride < head_dim)) || (heads > 1 && out_head_stride < head_dim))
     return ISP_ERR_SHAPE;
   if (!isp::aligned16(q) || !isp::aligned16(k) || !isp::aligned16(v) || !isp::aligned16(out)) return ISP_ERR_ALIGN;
   if (int st = isp::check_device()) return st;
@@ -1323,6 +1326,7 @@ int isp_paged_decode(const void* q, int dtype, int64_t q_seq_stride, int64_t q_h
   if (heads < 1 || heads > 65535 || heads % cache->kv_heads != 0 || B > 65535) return ISP_ERR_SHAPE;
   if (int st = check_strides(q_seq_stride, q_head_stride, 2)) return st;
   if (int st = check_strides(out_seq_stride, out_head_stride, 2)) return st;
+  if ((heads > 1 && out_head_stride < cache->head_dim) || (B > 1 && out_seq_stride < cache->head_dim)) return ISP_ERR_SHAPE;
   if (!isp::aligned16(q) || !isp::aligned16(out) || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
     return ISP_ERR_ALIGN;
   int64_t need = 0;

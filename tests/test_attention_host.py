@@ -50,6 +50,7 @@ def test_attention_refusals(lib):
     assert prompt(dtype=1) == 3
     assert prompt(dim=80) == 1 and prompt(heads=3) == 1 and prompt(kv=0) == 1 and prompt(b=-1) == 1 and prompt(tq=-1) == 1
     assert prompt(q=258) == 2 and prompt(qs=257) == 2
+    assert prompt(b=65537) == 1 and prompt(qs=0) == 1                    # too many sequences, overlapping rows
 
     def decode(cache=None, dtype=0, heads=4, scale=1.0, ws=256, size=1 << 30, qs=256):
         return lib.isp_paged_decode(256, dtype, qs, 64, ctypes.byref(cache or _cache()), 64, 4, 4, 64, 2, heads, scale,
