@@ -23,17 +23,18 @@
 //                   rows at the end.
 // Every wait is bounded; on expiry the block unwinds as the GEMMs do.
 //
-// Measured on one B200 (power-capped at 1.8 GHz in the long case): 16384 tokens, 32 over 8
-// heads of 128, 2.01 ms (1.09 PFLOP/s of causal work); 64 x 760 frames, 8 heads of 64, every
-// key, 139 us; 64 x 256 tokens, 20 heads of 64, 60.5 us.  Bound by the softmax: a step of both
-// tiles takes about 3700 cycles, of them 2048 in the special function unit and 1500 in the
-// tensor pipe; what is left is the chain S -> maximum -> exponentials -> PV of a tile.  Tried
-// and slower: half of the exponentials or fewer by polynomial (5 to 25%, the warps are bound by
-// their own instruction chains), a second read of S in a rolled loop (15%), two threads a row
-// (5 to 20% on long items), half of S(j + 1) before PV(j) (4%), no turns (10 to 18%).  The
-// roles' code has to stay small, they share the instruction cache: rolling the output and the
-// repair of non-finite values alone took 3 to 8% off, two scores to an instruction (f32x2) in
-// the products and sums of the exponentials another 3 to 9%.
+// Measured on one B200: 16384 tokens, 32 over 8 heads of 128, 2.04 ms call after call (at the
+// power cap; 1.08 PFLOP/s of causal work) and 1.78 ms alone; 64 x 760 frames, 8 heads of 64,
+// every key, 139 us; 64 x 256 tokens, 20 heads of 64, 55.7 us.  Bound by the softmax: a step of
+// both tiles takes about 3800 cycles, of them 2048 in the special function unit and as many in
+// the tensor pipe (each busy for 0.6 of the time); what is left is the chain S -> maximum ->
+// exponentials -> PV of a tile.  Tried and slower: half of the exponentials or fewer by
+// polynomial (5 to 25%, the warps are bound by their own instruction chains), a second read of
+// S in a rolled loop (15%; for masked tiles alone 3 to 7%), two threads a row (5 to 20% on long
+// items), half of S(j + 1) before PV(j) (4%), no turns (10 to 18%).  The roles' code has to stay
+// small, they share the instruction cache: rolling the output and the repair of non-finite
+// values alone took 3 to 8% off, two scores to an instruction (f32x2) in the products and sums
+// of the exponentials another 3 to 9%.
 #pragma once
 
 #include "gemm_sm100.cuh"
@@ -86,10 +87,11 @@ struct Item {
   int q0, rows;          // first query row, queries of the block
   int k0, keys;          // first key row, keys of the sequence
   int off;               // row r of the block sees the first min(keys, r + off + 1) keys
+  int swap;              // query tile t has the block's half t ^ swap
   int steps[2];          // key tiles of each query tile
   int edge;              // first key tile that some row does not see whole
   int flagged;           // the V check found non-finite values in view
-  int pad[5];
+  int pad[4];
 };
 
 struct Bars {
@@ -216,7 +218,8 @@ ISP_D void chunk_weights(const uint32_t (&s)[32], float scale, float base, float
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), make_float2(scale, scale), make_float2(-base, -base));
+    const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
+                                make_float2(scale, scale), make_float2(-base, -base));
     const float a = ex2(x.x), b = ex2(x.y);
     l[i & 1] = __fadd2_rn(l[i & 1], make_float2(a, b));
     w[i] = pack<kBf16>(a, b);
@@ -248,7 +251,7 @@ ISP_D int64_t blocks_from(const Params& p, int i, int lane) {
 }
 
 // Item number x in the order of falling block index (whole warp; `top`: blocks of the longest sequence).
-ISP_D void find_item(const Params& p, int64_t x, int top, int lane, Item& it) {
+ISP_D void find_item(const Params& p, int64_t x, int top, int swap, int lane, Item& it) {
   const int64_t block = x / p.heads;
   int lo = 0, hi = top - 1;                             // the largest i with blocks_from(i) > block
   while (lo < hi) {
@@ -283,12 +286,23 @@ ISP_D void find_item(const Params& p, int64_t x, int top, int lane, Item& it) {
   it.off = p.causal ? (it.q0 - q_first) + it.keys - (q_end - q_first) : it.keys;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int last = min(it.rows, (t + 1) * kTile) - 1;
-    const int seen = it.rows > t * kTile ? min(static_cast<int64_t>(it.keys), static_cast<int64_t>(last) + it.off + 1) : 0;
+    const int half = t ^ swap;
+    const int last = min(it.rows, (half + 1) * kTile) - 1;
+    const int seen = it.rows > half * kTile ? min(static_cast<int64_t>(it.keys), static_cast<int64_t>(last) + it.off + 1) : 0;
     it.steps[t] = max(0, (seen + kTile - 1) / kTile);
   }
   it.edge = max(0, min(it.keys, it.off < it.keys ? it.off + 1 : it.keys)) / kTile;
   it.flagged = 0;
+  it.swap = swap;
+}
+
+// 0 x + z of two 16-bit values each (one instruction for four of a test of the bits: 2.5% of 64 x 256 tokens).
+template <bool kBf16>
+ISP_D uint32_t times_zero(uint32_t x, uint32_t z) {
+  uint32_t r;
+  if constexpr (kBf16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(z));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(z));
+  return r;
 }
 
 // Whether one of two 16-bit values is infinite or NaN (exponent all ones).
@@ -367,7 +381,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const int64_t x = n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         Item it = {};
         it.stop = 1;
-        if (x < total) find_item(p, x, top, lane, it);
+        // The tiles take the halves of a block in alternation: in a causal block the second half
+        // has more keys, and in a short one the first is alone (64 x 256 tokens 57 us, with
+        // fixed halves 60 us; long items alike).
+        if (x < total) find_item(p, x, top, static_cast<int>(n & 1), lane, it);
         if (n >= kItemSlots && !gemm::wait_warp(&bars.item_free[slot], static_cast<uint32_t>((n / kItemSlots - 1) & 1), abort)) break;
         if (lane == 0) {
           bars.items[slot] = it;
@@ -388,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
               if (it.steps[t] == 0) continue;
               for (int c = 0; c < kD / 64; ++c)
                 gemm::tma_load_3d(smem + L::kQ + (buf * 2 + t) * L::kTileBytes + c * kTile * 128, &q_map, &bars.q_full[buf], c * 64,
-                                  it.head, it.q0 + t * kTile);
+                                  it.head, it.q0 + (t ^ it.swap) * kTile);
             }
           }
           __syncwarp();
@@ -530,12 +547,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           const uint32_t i = kv + 2 * j + 1, s = i % L::kStages;
           if (!(ok = gemm::wait_warp(&bars.v_in[edges & 3], (edges >> 2) & 1, abort))) break;
           uint8_t* tile = smem + L::kRing + s * L::kTileBytes;
-          uint32_t bad = 0;
+          uint32_t zero[4] = {0u, 0u, 0u, 0u};           // sums of 0 x: 0, or NaN for an infinity or NaN
 #pragma unroll 8
           for (int c = 0; c < L::kTileBytes / 512; ++c) {                // 4 rows of 128 bytes a step
             const uint4 w = *reinterpret_cast<const uint4*>(tile + c * 512 + lane * 16);
-            bad |= not_finite<kBf16>(w.x) | not_finite<kBf16>(w.y) | not_finite<kBf16>(w.z) | not_finite<kBf16>(w.w);
+            zero[0] = times_zero<kBf16>(w.x, zero[0]);
+            zero[1] = times_zero<kBf16>(w.y, zero[1]);
+            zero[2] = times_zero<kBf16>(w.z, zero[2]);
+            zero[3] = times_zero<kBf16>(w.w, zero[3]);
           }
+          const bool bad = not_finite<kBf16>(zero[0]) || not_finite<kBf16>(zero[1]) || not_finite<kBf16>(zero[2]) ||
+                           not_finite<kBf16>(zero[3]);
           if (__any_sync(0xffffffffu, bad)) {
             for (int c = 0; c < L::kTileBytes / 512; ++c) {
               const int row = (c % 32) * 4 + lane / 8;
@@ -566,7 +588,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const int t = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;        // TMEM lane quarter
     const uint32_t s_tmem = tmem + L::s(t) + lanes, o_tmem = tmem + L::o(t) + lanes;
-    const int row = t * kTile + (warp & 3) * 32 + lane;                  // row of the block
     const float slack = kSlack / p.scale;
     uint32_t s_count = 0, o_count = 0, turns = 0;                        // turns: of the other tile, in the items before
     bool ok = true;
@@ -576,9 +597,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       const Item& it = bars.items[slot];
       if (it.stop) break;
       const int steps = it.steps[t], steps_other = it.steps[t ^ 1];
+      const int first = (t ^ it.swap) * kTile, row = first + (warp & 3) * 32 + lane;   // rows of the block
       // keys that this row, and the tile's first row, see (<= 0: none)
       const int sees = static_cast<int>(min(static_cast<int64_t>(it.keys), static_cast<int64_t>(it.off) + row + 1));
-      const int whole = min(it.keys, it.off + t * kTile + 1);
+      const int whole = min(it.keys, it.off + first + 1);
       const bool take_turns = min(steps, steps_other) >= kTurnSteps;
       float m = -INFINITY, shift = 0.f, base = 0.f;                      // m in units of q.k
       bool far = false;
