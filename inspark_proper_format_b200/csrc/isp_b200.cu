@@ -1069,13 +1069,15 @@ Cache cache_of(const isp_kv_cache_t& c) {
                c.kv_heads, mul, 31 + s};
 }
 
-// About 256 rows a block (K and V of one token: 2 * heads rows), fewer where that would leave
+// Tokens of a block, for a grid of whole waves of `slots` blocks a multiprocessor and a row (K and
+// V of one token: 2 * heads rows) for each group of lanes, fewer where that would leave
 // multiprocessors without a block.
-int tokens_per_block(int heads, int64_t tokens) {
-  int64_t n = 128 / heads;
-  const int64_t spread = tokens / (4 * sm_count());
-  if (n > spread) n = spread;
-  return n < 1 ? 1 : static_cast<int>(n > kMaxTokensPerBlock ? kMaxTokensPerBlock : n);
+int tokens_per_block(int heads, int64_t tokens, int slots) {
+  const int64_t wave = static_cast<int64_t>(slots) * sm_count();
+  const int64_t waves = (tokens + wave * kMaxTokensPerBlock - 1) / (wave * kMaxTokensPerBlock);
+  const int64_t even = (tokens + waves * wave - 1) / (waves * wave);
+  const int64_t busy = std::min<int64_t>(32 / heads, tokens / (4 * sm_count()));
+  return static_cast<int>(std::max(even, busy));
 }
 
 template <int kD, int kIn>
@@ -1225,7 +1227,7 @@ int isp_kv_append(const void* k, const void* v, int x_dtype, int64_t T, int64_t 
   if (T == 0 || B == 0) return ISP_OK;
   RowParams p{cache_of(*cache), {page_table, table_stride, table_width, lengths, B}, cu_seqlens, T,
               {static_cast<uint8_t*>(const_cast<void*>(k)), static_cast<uint8_t*>(const_cast<void*>(v))},
-              {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, tokens_per_block(cache->kv_heads, T)};
+              {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, tokens_per_block(cache->kv_heads, T, append_blocks(cache->dtype))};
   const unsigned grid = static_cast<unsigned>((T + p.tokens_per_block - 1) / p.tokens_per_block);
   return cache->head_dim == 64 ? append<64>(p, x_dtype, cache->dtype, grid, stream)
                                : append<128>(p, x_dtype, cache->dtype, grid, stream);
@@ -1246,7 +1248,7 @@ int isp_kv_gather(const isp_kv_cache_t* cache, const int32_t* cu_seqlens, const 
   const int64_t head = cache->head_dim, token = head * cache->kv_heads;
   RowParams p{cache_of(*cache), {page_table, table_stride, table_width, lengths, B}, cu_seqlens, T,
               {static_cast<uint8_t*>(k_out), static_cast<uint8_t*>(v_out)}, {token, token}, {head, head},
-              tokens_per_block(cache->kv_heads, T)};
+              tokens_per_block(cache->kv_heads, T, kGatherBlocks)};
   const unsigned grid = static_cast<unsigned>((T + p.tokens_per_block - 1) / p.tokens_per_block);
   return cache->head_dim == 64 ? gather<64>(p, cache->dtype, out_dtype, grid, stream)
                                : gather<128>(p, cache->dtype, out_dtype, grid, stream);

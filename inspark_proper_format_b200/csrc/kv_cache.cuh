@@ -174,6 +174,10 @@ ISP_D uint4 f32_to_codes16(const float (&x)[16]) {
 ISP_HD constexpr int type_bytes(int t) { return t == ISP_F32 ? 4 : (t == ISP_BF16 || t == ISP_F16 ? 2 : 1); }
 ISP_HD constexpr bool is_code(int t) { return t == ISP_E4M3 || t == ISP_I8; }
 
+// Blocks of a multiprocessor: append in one wave, gather in four of eight.
+ISP_HD constexpr int append_blocks(int code) { return is_code(code) ? 6 : 8; }
+constexpr int kGatherBlocks = 32;
+
 struct RowParams {
   Cache cache;
   Table table;
@@ -231,15 +235,18 @@ struct RowWalk {
   }
 };
 
-// Both kernels are bound by the bytes they move: 16 elements a lane (8 for 16-bit caches),
-// kD / 16 lanes a row, blocks of 256 rows or so (fewer where the call has few tokens), so that
-// the look-up of a block's tokens is a small part of it (64 rows 1 to 50% slower, 1024 rows
-// 30%).  One row a lane at a time: two or four in flight cost registers, and with them more
+// Both kernels are bound by the bytes they move: 16 elements a lane (8 for 16-bit caches) and
+// kD / 16 lanes a row.  A block starts with the look-up of its tokens, three dependent loads.
+// Append takes one wave of equal blocks, as many as its registers leave room for (16384 tokens,
+// 20 heads of 64: INT8 32.7 us, in blocks of 256 rows 36.4, in more than one wave 36 to 43;
+// BF16 rows 33.3 us, 37.5 in such blocks); gather, with less work a row, four waves, so that
+// some blocks look up while others move (2% faster than blocks of 256 rows, 7% than one
+// wave).  One row a lane at a time: two or four in flight cost registers, and with them more
 // than they hid (10 and 45%).  Measured, append then gather on one B200: INT8, 64 x 256
-// tokens, 20 heads of 64, 65 us (4.0 TB/s of 257 MB); E4M3, 44246 tokens, 8 heads of 128,
-// 115 us (4.8 TB/s of 549 MB).
+// tokens, 20 heads of 64, 59.5 us (4.3 TB/s of 257 MB); E4M3, 44246 tokens, 8 heads of 128,
+// 110 us (5.0 TB/s of 549 MB).
 template <int kD, int kIn, int kCode>
-__global__ void __launch_bounds__(kRowThreads) append_kernel(const RowParams p) {
+__global__ void __launch_bounds__(kRowThreads, append_blocks(kCode)) append_kernel(const RowParams p) {
   constexpr int kElems = is_code(kCode) ? 16 : 8, kLanes = kD / kElems;
   __shared__ int64_t rows[kMaxTokensPerBlock];
   __shared__ int bounds[kBoundsAtOnce + 1];
