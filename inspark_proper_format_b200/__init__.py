@@ -2,7 +2,8 @@
 
 Torch-level ops over the C ABI in ``include/isp_b200.h``:
 norm->quantize, W8A8 FP8/INT8 scaled GEMMs with fused epilogues, the CFM
-gated-up SwiGLU and the BigVGAN anti-aliased Snake FIR.  Every op runs a
+gated-up SwiGLU, the BigVGAN anti-aliased Snake FIR, and serving attention
+(paged quantised key-value cache, packed prompts, decode).  Every op runs a
 hand-written CUDA kernel; there is no CPU fallback.
 """
 from . import _lib  # noqa: F401

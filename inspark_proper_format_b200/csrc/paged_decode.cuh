@@ -32,7 +32,7 @@
 // to 16 bits (FP16 over 8-bit and FP16 rows, BF16 over BF16 rows); sums are FP32.
 //
 // Measured on one B200, cold inputs: INT8, head_dim 128, 32 over 8 heads, 238651 cached
-// tokens 97.7 us (5.16 TB/s); FP16, the same heads, 37 sequences of up to 6000 tokens 29.0 us
+// tokens 100 us (5.0 TB/s); FP16, the same heads, 37 sequences of up to 6000 tokens 29.0 us
 // (3.27 TB/s); E4M3, head_dim 64, 20 heads, 64 sequences of 256 to 2048 tokens 43.7 us
 // (3.47 TB/s), bound by latency in the warps' unpacking rather than by the copies, which
 // alone take 29 us.
