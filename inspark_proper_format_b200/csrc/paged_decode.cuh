@@ -25,16 +25,17 @@
 // exactly; the order of a row's elements inside a product is free, so each lane takes the
 // 16 bytes it loads as its fragment, with keys in the order of key_row() that makes K's
 // rows V's columns and keeps both reads free of bank conflicts.  Their scales go to the
-// FP32 scores (K) and to p (V): p carries a power of two that follows the largest v_scale
-// seen and keeps p * v_scale below 2^15, so FP16 resolves it down to 2^-28 of the largest
-// weight.  BF16 queries over 8-bit rows are brought into FP16's range by a power of two per
-// head and are exact there down to 2^-38 of the head's largest element.  p is rounded once
-// to 16 bits (FP16 over 8-bit and FP16 rows, BF16 over BF16 rows); sums are FP32.
+// FP32 scores (K) and to p (V): p * v_scale carries a power of two that follows its largest
+// value so far and keeps that between 2^6 and 2^15, so FP16 has all its bits down to 2^-20 of
+// the largest p * v_scale and loses what lies below 2^-31 of it.  BF16 queries over 8-bit rows
+// are brought into FP16's range by a power of two per head and keep all their bits down to
+// 2^-31 of the head's largest element; below 2^-39 of it they are lost.  p is rounded once to 16
+// bits (FP16 over 8-bit and FP16 rows, BF16 over BF16 rows); sums are FP32.
 //
 // Measured on one B200, cold inputs: INT8, head_dim 128, 32 over 8 heads, 238651 cached
 // tokens 100 us (5.0 TB/s); FP16, the same heads, 37 sequences of up to 6000 tokens 29.0 us
-// (3.27 TB/s); E4M3, head_dim 64, 20 heads, 64 sequences of 256 to 2048 tokens 43.7 us
-// (3.47 TB/s), bound by latency in the warps' unpacking rather than by the copies, which
+// (3.27 TB/s); E4M3, head_dim 64, 20 heads, 64 sequences of 256 to 2048 tokens 44.9 us
+// (3.38 TB/s), bound by latency in the warps' unpacking rather than by the copies, which
 // alone take 29 us.
 #pragma once
 
@@ -55,13 +56,18 @@ struct DecodeParams {
   int gb;                 // query heads of a full block: min(group, 8)
   float scale;            // softmax scale * log2(e)
   unsigned* counters;     // [kMaxBlocks], zero between calls
-  float* partials;        // [2 * kMaxBlocks] pieces: [8][head_dim] weighted sums, [8] {m, l}
+  float* partials;        // [2 * kMaxBlocks] pieces: [8][head_dim] weighted sums, [8] Refs
 };
 
 constexpr int kDecWarps = 4;
 constexpr int kMaxBlocks = 1024;
-constexpr int kSlotFloats = 8 * (128 + 2);
+constexpr int kSlotFloats = 8 * (128 + 4);
 constexpr int64_t kDecWorkspace = kMaxBlocks * 4ll + 2ll * kMaxBlocks * kSlotFloats * 4;
+
+// log2 of what a weighted sum and a sum of weights are in units of, and the sum of weights
+struct __align__(16) Refs {
+  float o, m, l, unused;
+};
 
 ISP_D void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -169,7 +175,7 @@ struct Tile {
   // stage: K rows, V rows, per row {K scale, V scale}, the valid mask
   static constexpr int kV = kT * kRow, kScales = 2 * kV, kMask = kScales + 8 * kT, kBytesPerStage = kMask + 16;
   static constexpr int kRing = kDecWarps * kStages * kBytesPerStage;
-  static constexpr int smem_bytes(int gb) { return kRing + kDecWarps * gb * (kD + 2) * 4; }
+  static constexpr int smem_bytes(int gb) { return kRing + kDecWarps * gb * (kD + 4) * 4; }
 };
 
 // 16-byte chunk c of row r lies at chunk c ^ swizzle(r), so that the 8 lanes of a 16-byte
@@ -228,8 +234,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
   __shared__ unsigned arrived;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * kStages * T::kBytesPerStage;
-  float* joins = reinterpret_cast<float*>(smem + T::kRing);   // [warp][gb][kD] weighted sums, [warp][gb] {m, l}
-  float2* joins_ml = reinterpret_cast<float2*>(joins + kDecWarps * p.gb * kD);
+  float* joins = reinterpret_cast<float*>(smem + T::kRing);   // [warp][gb][kD] weighted sums, [warp][gb] Refs
+  Refs* joins_refs = reinterpret_cast<Refs*>(joins + kDecWarps * p.gb * kD);
   const int hgs = p.cache.heads * p.gblocks;
   pdl_wait();
   pdl_trigger();
@@ -398,17 +404,23 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
 
   uint32_t qb[kKSteps][2];
   float q_unit[2] = {p.scale, p.scale};                // heads 2t, 2t + 1: softmax scale over the power of two in qb
-  // p = 2^(s - m + v_up): m follows the maximum of s (heads 2t, 2t + 1), v_up the largest
-  // v_scale.  m may stay up to kSlack behind, so that most tiles rescale nothing.
-  constexpr float kSlack = 8.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, v_up = 0.f, v_ref = 0.f;           // l: this lane's keys only; v_ref: above every v_scale so far
+  // Heads 2t and 2t + 1.  l = sum of p = 2^(s - m) over this lane's keys, m following the maximum
+  // of s.  Over 8-bit rows p * v_scale enters the product with V as p * v_scale * c, c = 2^(m - r +
+  // kUp), where r follows the largest s + log2(v_scale): the largest weight in use lies in (2^(kUp
+  // - 1), 2^15], whatever the scales of rows are whose own weight is small.  Either reference may
+  // stay up to kSlack behind, so that most tiles rescale nothing.
+  constexpr float kSlack = 8.f, kUp = 15.f - kSlack;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, r[2] = {-INFINITY, -INFINITY}, c[2] = {0.f, 0.f};
+  // log2 of |v_scale|, rounded up; scales under 2^-64 are not brought up
+  const auto log2_above = [](float v) { return fmaxf(static_cast<float>(static_cast<int>((__float_as_uint(v) >> 23) & 255u) - 126), -64.f); };
   float o[kOBlocks][4];
 
   for (int u = 0; u < count; ++u) {
     if (u == 0 || at.step == 0) {                      // a new item
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
-      v_ref = 0.f;
+      r[0] = r[1] = -INFINITY;
+      c[0] = c[1] = 0.f;
 #pragma unroll
       for (int i = 0; i < kOBlocks; ++i)
 #pragma unroll
@@ -506,48 +518,53 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
       }
     }
 
-    // ---- references: move them when a score or a v_scale passes them ----
+    // ---- references: move them when a score or a product passes them ----
     float top[2] = {s[0][0], s[0][1]};
 #pragma unroll
     for (int kb = 0; kb < kKeyBlocks; ++kb) {
       top[0] = fmaxf(top[0], fmaxf(s[kb][0], s[kb][2]));
       top[1] = fmaxf(top[1], fmaxf(s[kb][1], s[kb][3]));
     }
-    float v_top = 0.f;
+    bool past = top[0] > m[0] + kSlack || top[1] > m[1] + kSlack;
     if constexpr (kIsCode) {
+      float v_top = 0.f;                               // a NaN scale is dropped: its row's weight is NaN anyway
 #pragma unroll
-      for (int kb = 0; kb < kKeyBlocks; ++kb) v_top = fmaxf(v_top, fmaxf(f[kb][0].y, f[kb][1].y));
+      for (int kb = 0; kb < kKeyBlocks; ++kb) v_top = fmaxf(v_top, fmaxf(fabsf(f[kb][0].y), fabsf(f[kb][1].y)));
+      const float above = log2_above(v_top);           // top + above: no product of this lane lies higher
+      past = past || top[0] + above > r[0] + kSlack || top[1] + above > r[1] + kSlack;
     }
-    const bool past = top[0] > m[0] + kSlack || top[1] > m[1] + kSlack || v_top > v_ref;
     if (__any_sync(0xffffffffu, past)) {
-      float keep[2];
-      const float v_old = v_up;
-      if constexpr (kIsCode) {
-        // positive floats compare as integers (a NaN scale was dropped by fmaxf: its row's weight is NaN anyway)
-        const unsigned all = __reduce_max_sync(0xffffffffu, __float_as_uint(v_top));
-        if (__uint_as_float(all) > v_ref) {
-          // four times the scale, rounded up to a power of two: later rows seldom pass it.
-          // p * v_scale < 2^(kSlack + v_up) * v_ref = 2^15; scales under 2^-64 are not brought up
-          const unsigned e = min(max((all >> 23) + 3u, 127u - 64u), 254u);
-          v_ref = __uint_as_float(e << 23);
-          v_up = 15.f - kSlack + 127.f - static_cast<float>(e);
-        }
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        float product = -INFINITY;                     // the largest s + log2(v_scale)
+        if constexpr (kIsCode) {
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
-        const float m_old = m[h];
+          for (int kb = 0; kb < kKeyBlocks; ++kb)
+            product = fmaxf(product, fmaxf(s[kb][h] + log2_above(f[kb][0].y), s[kb][2 + h] + log2_above(f[kb][1].y)));
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+          if constexpr (kIsCode) product = fmaxf(product, __shfl_xor_sync(0xffffffffu, product, d));
+        }
+        const float m_old = m[h], r_old = r[h];
         if (top[h] > m[h] + kSlack) m[h] = top[h];
-        keep[h] = m_old == -INFINITY ? 0.f : exp2_approx((m_old - m[h]) + (v_up - v_old));
-        l[h] *= keep[h];
+        const float keep_l = m_old == -INFINITY ? 0.f : exp2_approx(m_old - m[h]);
+        float keep_o = keep_l;
+        l[h] *= keep_l;
+        if constexpr (kIsCode) {
+          if (product > r[h] + kSlack) r[h] = product;
+          keep_o = r_old == -INFINITY ? 0.f : exp2_approx(r_old - r[h]);
+          c[h] = r[h] == -INFINITY ? 0.f : exp2_approx(m[h] - r[h] + kUp);
+        }
+#pragma unroll
+        for (int i = 0; i < kOBlocks; ++i) {
+          o[i][h] *= keep_o;
+          o[i][2 + h] *= keep_o;
+        }
       }
-#pragma unroll
-      for (int i = 0; i < kOBlocks; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] *= keep[j & 1];
     }
-    const float base[2] = {(m[0] == -INFINITY ? 0.f : m[0]) - v_up, (m[1] == -INFINITY ? 0.f : m[1]) - v_up};
+    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 
     // ---- weights and their product with V, 16 keys at a time ----
 #pragma unroll
@@ -557,7 +574,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
       for (int j = 0; j < 4; ++j) {
         w[j] = exp2_approx(s[kb][j] - base[j & 1]);
         l[j & 1] += w[j];
-        if constexpr (kIsCode) w[j] *= f[kb][j >> 1].y;
+        if constexpr (kIsCode) w[j] = w[j] * c[j & 1] * f[kb][j >> 1].y;
       }
       const uint32_t b0 = transpose8x8(pack16<kMmaBf16>(w[0], w[1]));
       const uint32_t b1 = transpose8x8(pack16<kMmaBf16>(w[2], w[3]));
@@ -609,31 +626,34 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
             joins[mine * kD + d0] = o[j][h];
             joins[mine * kD + d0 + (kIsCode ? 1 : 8)] = o[j][2 + h];
           }
-          if (g == 0) joins_ml[mine] = make_float2(m[h] - v_up, l[h]);
+          if (g == 0) joins_refs[mine] = {kIsCode ? r[h] - kUp : m[h], m[h], l[h], 0.f};
         }
       }
       __syncthreads();
       const int hk = at.hg / p.gblocks, head0 = hk * p.group + (at.hg % p.gblocks) * 8;
       const int n = min(8, p.group - (at.hg % p.gblocks) * 8);
       const int64_t begin = u0 + u - at.step, end = begin + at.steps;   // the item's units
-      // the four sums in shared memory as one: the result, or this run's piece of it
+      // the four sums in shared memory as one: the result, or this run's piece of it.  Weighted sums and
+      // sums of weights are added in units of their own, which meet in the quotient.
+      const auto or_zero = [](float x) { return x == -INFINITY ? 0.f : x; };
       const auto join = [&](float* slot) {
         for (int i = threadIdx.x; i < n * (kD / 4); i += kDecWarps * 32) {
           const int h = i / (kD / 4), d = i % (kD / 4) * 4;
-          float2 ml[kDecWarps];
-          float top = -INFINITY, sum = 0.f;
+          Refs refs[kDecWarps];
+          Refs top = {-INFINITY, -INFINITY, 0.f, 0.f};
 #pragma unroll
           for (int w = 0; w < kDecWarps; ++w) {
-            ml[w] = joins_ml[w * p.gb + h];
-            top = fmaxf(top, ml[w].x);
+            refs[w] = joins_refs[w * p.gb + h];
+            top.o = fmaxf(top.o, refs[w].o);
+            top.m = fmaxf(top.m, refs[w].m);
           }
-          const float ref = top == -INFINITY ? 0.f : top;
+          const float ref_o = or_zero(top.o), ref_m = or_zero(top.m);
           float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int w = 0; w < kDecWarps; ++w) {
-            const float f = exp2_approx(ml[w].x - ref);
+            const float f = exp2_approx(refs[w].o - ref_o);
             const float4 x = *reinterpret_cast<const float4*>(joins + (w * p.gb + h) * kD + d);
-            sum += f * ml[w].y;
+            top.l += (kIsCode ? exp2_approx(refs[w].m - ref_m) : f) * refs[w].l;
             r.x += f * x.x;
             r.y += f * x.y;
             r.z += f * x.z;
@@ -641,11 +661,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
           }
           if (slot != nullptr) {
             __stcg(reinterpret_cast<float4*>(slot + h * kD + d), r);
-            if (d == 0) __stcg(reinterpret_cast<float2*>(slot + 8 * kD) + h, make_float2(top, sum));
+            if (d == 0) __stcg(reinterpret_cast<float4*>(slot + 8 * kD) + h, make_float4(top.o, top.m, top.l, 0.f));
           } else {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const float inv = top.l == 0.f ? 0.f : 1.f / top.l, unit = kIsCode ? exp2_approx(ref_o - ref_m) : 1.f;
             uint8_t* dst = p.out + (at.b * p.o_seq + (head0 + h) * p.o_head + d) * 2;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<kQBf16>(r.x * inv, r.y * inv), pack16<kQBf16>(r.z * inv, r.w * inv));
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<kQBf16>(r.x * inv * unit, r.y * inv * unit),
+                                                        pack16<kQBf16>(r.z * inv * unit, r.w * inv * unit));
           }
         }
       };
@@ -666,61 +687,60 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
           constexpr int kLanes = kD / 4, kGroups = kDecWarps * 32 / kLanes;
           const int group = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
           for (int h = 0; h < n; ++h) {
-            float top = -INFINITY, sum = 0.f;
+            Refs top = {-INFINITY, -INFINITY, 0.f, 0.f};
             float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-            const auto add = [&](float2 ml, float4 x, float ref) {
-              const float f = exp2_approx(ml.x - ref);
-              sum += f * ml.y;
-              r.x += f * x.x;
-              r.y += f * x.y;
-              r.z += f * x.z;
-              r.w += f * x.w;
-            };
-            for (int64_t b = b0 + group; b <= b1; b += 4 * kGroups) {
-              float2 ml[4];
-              float4 x[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int64_t bi = b + i * kGroups;
-                ml[i] = make_float2(-INFINITY, 0.f);
-                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (bi <= b1) {
-                  const float* src = p.partials + (2 * bi + (bi == b0 ? 1 : 0)) * kSlotFloats;
-                  ml[i] = __ldcg(reinterpret_cast<const float2*>(src + 8 * kD) + h);
-                  x[i] = __ldcg(reinterpret_cast<const float4*>(src + h * kD + d));
-                }
-              }
-              const float now = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top);
-              const float ref = now == -INFINITY ? 0.f : now;
-              const float keep = exp2_approx(top - ref);
-              sum *= keep;
-              r.x *= keep;
-              r.y *= keep;
-              r.z *= keep;
-              r.w *= keep;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) add(ml[i], x[i], ref);
-              top = now;
-            }
-            if constexpr (kLanes == 16) {              // the warp's two groups
-              const float other = __shfl_xor_sync(0xffffffffu, top, 16);
-              const float now = fmaxf(top, other), ref = now == -INFINITY ? 0.f : now;
-              const float f = exp2_approx(top - ref);
-              sum *= f;
+            const auto scale = [&](float f, float f_l) {
+              top.l *= f_l;
               r.x *= f;
               r.y *= f;
               r.z *= f;
               r.w *= f;
-              sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            };
+            for (int64_t b = b0 + group; b <= b1; b += 4 * kGroups) {
+              float4 refs[4], x[4];                    // Refs
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int64_t bi = b + i * kGroups;
+                refs[i] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (bi <= b1) {
+                  const float* src = p.partials + (2 * bi + (bi == b0 ? 1 : 0)) * kSlotFloats;
+                  refs[i] = __ldcg(reinterpret_cast<const float4*>(src + 8 * kD) + h);
+                  x[i] = __ldcg(reinterpret_cast<const float4*>(src + h * kD + d));
+                }
+              }
+              const float now_o = fmaxf(fmaxf(fmaxf(refs[0].x, refs[1].x), fmaxf(refs[2].x, refs[3].x)), top.o);
+              const float now_m = kIsCode ? fmaxf(fmaxf(fmaxf(refs[0].y, refs[1].y), fmaxf(refs[2].y, refs[3].y)), top.m) : now_o;
+              const float ref_o = or_zero(now_o), ref_m = or_zero(now_m), keep = exp2_approx(top.o - ref_o);
+              scale(keep, kIsCode ? exp2_approx(top.m - ref_m) : keep);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float f = exp2_approx(refs[i].x - ref_o);
+                top.l += (kIsCode ? exp2_approx(refs[i].y - ref_m) : f) * refs[i].z;
+                r.x += f * x[i].x;
+                r.y += f * x[i].y;
+                r.z += f * x[i].z;
+                r.w += f * x[i].w;
+              }
+              top.o = now_o;
+              top.m = now_m;
+            }
+            if constexpr (kLanes == 16) {              // the warp's two groups
+              const float now_o = fmaxf(top.o, __shfl_xor_sync(0xffffffffu, top.o, 16));
+              const float now_m = kIsCode ? fmaxf(top.m, __shfl_xor_sync(0xffffffffu, top.m, 16)) : now_o;
+              const float f = exp2_approx(top.o - or_zero(now_o));
+              scale(f, kIsCode ? exp2_approx(top.m - or_zero(now_m)) : f);
+              top.l += __shfl_xor_sync(0xffffffffu, top.l, 16);
               r.x += __shfl_xor_sync(0xffffffffu, r.x, 16);
               r.y += __shfl_xor_sync(0xffffffffu, r.y, 16);
               r.z += __shfl_xor_sync(0xffffffffu, r.z, 16);
               r.w += __shfl_xor_sync(0xffffffffu, r.w, 16);
-              top = now;
+              top.o = now_o;
+              top.m = now_m;
             }
             if (lane < kLanes) {
               *reinterpret_cast<float4*>(joins + (warp * p.gb + h) * kD + d) = r;
-              if (lane == 0) joins_ml[warp * p.gb + h] = make_float2(top, sum);
+              if (lane == 0) joins_refs[warp * p.gb + h] = top;
             }
           }
           __syncthreads();

@@ -1,0 +1,83 @@
+"""GPU: attention over rows of very different sizes, against the definition in 64 bits
+(tests/attention_f64.py)."""
+import numpy as np
+import pytest
+import torch
+
+from attention_f64 import attend, check
+from test_gpu_attention import _cu, _i32, _randn, check_decode, make_cache
+from test_gpu_kv_cache import layout
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def at():
+    from inspark_proper_format_b200 import attention
+    return attention
+
+
+@pytest.fixture(scope="module")
+def kv():
+    from inspark_proper_format_b200 import kv_cache
+    return kv_cache
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    from inspark_proper_format_b200 import _lib
+    _lib.read_device_error(clear=True)
+    yield
+    assert _lib.read_device_error(clear=True) == 0
+
+
+def cache_of(kv, k, v, lens, page, fmt, seed):
+    """A cache that holds these rows, its page table, and (k, v) as it reads them back."""
+    table, pages = layout(lens, page, seed)
+    cache = kv.PagedKVCache(pages, k.shape[1], k.shape[2], page_size=page, fmt=fmt)
+    kv.kv_append(cache, k, v, table, _i32(lens), _cu(lens))
+    return cache, table, kv.kv_gather(cache, table, _i32(lens), _cu(lens), tokens=sum(lens), dtype=torch.float32)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,heads,kv_heads,page", [([9], 1, 1, 16), ([700, 40], 8, 2, 16), ([5000], 4, 4, 64)])
+def test_decode_one_large_value_row(at, kv, lens, heads, kv_heads, page, dim, dtype, fmt):
+    """One key's values are 2^up larger than the others' and its weight 2^-drop of theirs: it adds
+    up to as much as they do, or nothing that counts, and takes nothing from what they add,
+    wherever it stands in the sequence."""
+    q = _randn(len(lens), heads, dim, seed=100, dtype=dtype, gain=0.5)
+    q[..., 0] = 1.0
+    k = _randn(sum(lens), kv_heads, dim, seed=101, dtype=torch.float32)
+    k[..., 0] = 0.0
+    v = _randn(sum(lens), kv_heads, dim, seed=102, dtype=torch.float32)
+    first = np.concatenate([[0], np.cumsum(lens)[:-1]])
+    for drop, up in ((80, 22), (80, 26), (80, 28), (80, 30), (80, 32), (80, 60), (30, 30), (80, 84)):
+        for where in (0.0, 0.5, 1.0):
+            kk, vv = k.clone(), v.clone()
+            for a, n in zip(first, lens):
+                row = int(a + where * (n - 1))
+                kk[row] = 0.0
+                kk[row, :, 0] = -drop * np.log(2.0) * dim ** 0.5       # the score is -drop log 2
+                vv[row] *= 2.0 ** up
+            cache, table, back = cache_of(kv, kk, vv, lens, page, fmt, 103)
+            check_decode(at.paged_decode_attention(q, cache, table, _i32(lens)), q, back, lens)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+def test_decode_value_rows_over_32_octaves(at, kv, order, fmt):
+    """V rows whose scales span 2^32, each at a score of its own."""
+    lens, dim = [3000, 257], 64
+    q = _randn(2, 8, dim, seed=110, dtype=torch.bfloat16, gain=2.0)
+    k = _randn(sum(lens), 2, dim, seed=111, dtype=torch.float32)
+    v = _randn(sum(lens), 2, dim, seed=112, dtype=torch.float32)
+    octaves = torch.cat([torch.linspace(-16, 16, n) for n in lens])
+    if order == "falling":
+        octaves = -octaves
+    elif order == "mixed":
+        octaves = octaves[torch.randperm(sum(lens), generator=torch.Generator().manual_seed(113))]
+    v *= torch.exp2(octaves.round())[:, None, None].cuda()
+    cache, table, back = cache_of(kv, k, v, lens, 64, fmt, 114)
+    check_decode(at.paged_decode_attention(q, cache, table, _i32(lens)), q, back, lens)
