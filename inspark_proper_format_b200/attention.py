@@ -109,7 +109,7 @@ def paged_decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: tor
         raise ValueError("q does not fit the cache's head_dim and kv_heads")
     if cache.k_scale is None and cache.dtype != q.dtype:
         raise ValueError("a 16-bit cache must have the queries' type")
-    table = table_args(page_table, lengths, q.device)
+    table, page_table = table_args(page_table, lengths, q.device)
     if table[-1] != q.shape[0]:
         raise ValueError("page_table and lengths must have one row per query")
     value = _softmax_scale(scale, q.shape[2])

@@ -94,7 +94,9 @@ def index_array(t: torch.Tensor, name: str, device, size=None) -> int:
 
 
 def table_args(page_table: torch.Tensor, lengths: torch.Tensor, device):
-    """(pointer, row stride, width, lengths pointer, batch) of a page table and its lengths."""
+    """((pointer, row stride, width, lengths pointer, batch), table) of a page table and its lengths.
+    The kernels step from row to row by at least the width, so a view whose rows overlap (an
+    expanded one) is copied; the caller keeps ``table`` until the call."""
     if (not isinstance(page_table, torch.Tensor) or page_table.dtype is not torch.int32 or not page_table.is_cuda
             or page_table.device != device or page_table.ndim != 2):
         raise ValueError("page_table must be an int32 CUDA tensor [batch, pages per sequence]")
@@ -102,7 +104,11 @@ def table_args(page_table: torch.Tensor, lengths: torch.Tensor, device):
     stride, last = page_table.stride()
     if width < 1 or (last != 1 and width > 1):
         raise ValueError("page_table must be an int32 CUDA tensor [batch, pages per sequence]")
-    return page_table.data_ptr(), max(stride, width), width, index_array(lengths, "lengths", device, batch), batch
+    if stride < width and batch > 1:
+        page_table = page_table.contiguous()
+    args = (page_table.data_ptr(), max(page_table.stride(0), width), width,
+            index_array(lengths, "lengths", device, batch), batch)
+    return args, page_table
 
 
 def call(device, name: str, *args) -> None:
@@ -142,7 +148,7 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_table:
         raise ValueError("k and v must both be [tokens, kv_heads, head_dim] of the cache")
     if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError("k and v must both be BF16, FP16 or FP32")
-    table = table_args(page_table, lengths, cache.device)
+    table, page_table = table_args(page_table, lengths, cache.device)
     cu = None
     if cu_seqlens is not None:
         cu = index_array(cu_seqlens, "cu_seqlens", cache.device, table[-1] + 1)
@@ -164,7 +170,7 @@ def kv_gather(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tens
     positions before a sequence's start, are zeros."""
     if dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError("rows are read back as BF16, FP16 or FP32")
-    table = table_args(page_table, lengths, cache.device)
+    table, page_table = table_args(page_table, lengths, cache.device)
     batch = table[-1]
     cu = None
     if cu_seqlens is None:
