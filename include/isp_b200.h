@@ -449,7 +449,8 @@ int isp_kv_gather(const isp_kv_cache_t *cache, const int32_t *cu_seqlens,
  * or ISP_F16), out like q in the same type; strides in elements as in isp_kv_append.
  * cu_seqlens_q, cu_seqlens_k: int32 [B + 1] device arrays as above.  head_dim 64 or 128,
  * heads % kv_heads == 0, scale finite and positive, B <= 65536, fewer than 2^30 tokens,
- * k_tokens >= 1; rows must not overlap (no zero strides).
+ * k_tokens >= 1; strides of at least head_dim, and no two rows of `out` share an element
+ * (ISP_ERR_SHAPE).
  */
 int isp_prompt_attention(const void *q, const void *k, const void *v, int dtype,
                          int64_t q_tokens, int64_t k_tokens,
@@ -466,7 +467,7 @@ int isp_prompt_attention(const void *q, const void *k, const void *v, int dtype,
  * Attention of one token per sequence over the paged cache: q, out: [B, heads, head_dim] in
  * `dtype` (ISP_BF16 or ISP_F16), strides as above; the token sees positions
  * [0, lengths[b]) (its own row is appended before); length 0 gives zeros.  A 16-bit cache
- * has q's type.  B <= 65535.
+ * has q's type.  B <= 65535; no two rows of `out` share an element (ISP_ERR_SHAPE).
  *
  * workspace: isp_paged_decode_workspace bytes of device memory, 256-byte aligned, zero
  * before its first use; every call leaves it ready for the next one on the same stream.

@@ -3,6 +3,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <utility>
 
 #include "common.cuh"
 #include "conv.cuh"
@@ -1061,6 +1062,23 @@ int check_strides(int64_t a, int64_t b, int bytes) {
   return (a * bytes % 16 || b * bytes % 16) ? ISP_ERR_ALIGN : ISP_OK;
 }
 
+// Whether two of na x nb rows of `dim` elements share one: rows i apart along a and j along b, to the
+// same or opposite sides, with |i sa -+ j sb| < dim.
+bool rows_overlap(int64_t na, int64_t sa, int64_t nb, int64_t sb, int dim) {
+  if (na <= 1 && nb <= 1) return false;
+  if (na < nb) {
+    std::swap(na, nb);
+    std::swap(sa, sb);
+  }
+  if (sa < dim || (nb > 1 && sb < dim)) return true;
+  if (sa >= (nb - 1) * sb + dim || sb >= (na - 1) * sa + dim) return false;   // one dimension inside a step of the other
+  for (int64_t j = 1; j < nb; ++j) {
+    const int64_t i = j * sb / sa, left = j * sb - i * sa;                     // left < sa
+    if ((i < na && left < dim) || (i + 1 < na && sa - left < dim)) return true;
+  }
+  return false;
+}
+
 Cache cache_of(const isp_kv_cache_t& c) {
   int s = 0;
   while ((1ll << s) < c.page_size) ++s;
@@ -1271,10 +1289,10 @@ int isp_prompt_attention(const void* q, const void* k, const void* v, int dtype,
   if (int st = check_strides(k_token_stride, k_head_stride, 2)) return st;
   if (int st = check_strides(v_token_stride, v_head_stride, 2)) return st;
   if (int st = check_strides(out_token_stride, out_head_stride, 2)) return st;
-  // rows of a tensor map, and those of the output, do not overlap
+  // strides of a tensor map, and rows of the output that different blocks write
   if ((heads > 1 && q_head_stride < head_dim) || (kv_heads > 1 && (k_head_stride < head_dim || v_head_stride < head_dim)) ||
-      (k_tokens > 1 && (k_token_stride < head_dim || v_token_stride < head_dim)) ||
-      (q_tokens > 1 && (q_token_stride < head_dim || out_token_stride < head_dim)) || (heads > 1 && out_head_stride < head_dim))
+      (k_tokens > 1 && (k_token_stride < head_dim || v_token_stride < head_dim)) || (q_tokens > 1 && q_token_stride < head_dim) ||
+      rows_overlap(q_tokens, out_token_stride, heads, out_head_stride, head_dim))
     return ISP_ERR_SHAPE;
   if (!isp::aligned16(q) || !isp::aligned16(k) || !isp::aligned16(v) || !isp::aligned16(out)) return ISP_ERR_ALIGN;
   if (int st = isp::check_device()) return st;
@@ -1328,7 +1346,7 @@ int isp_paged_decode(const void* q, int dtype, int64_t q_seq_stride, int64_t q_h
   if (heads < 1 || heads > 65535 || heads % cache->kv_heads != 0 || B > 65535) return ISP_ERR_SHAPE;
   if (int st = check_strides(q_seq_stride, q_head_stride, 2)) return st;
   if (int st = check_strides(out_seq_stride, out_head_stride, 2)) return st;
-  if ((heads > 1 && out_head_stride < cache->head_dim) || (B > 1 && out_seq_stride < cache->head_dim)) return ISP_ERR_SHAPE;
+  if (rows_overlap(B, out_seq_stride, heads, out_head_stride, cache->head_dim)) return ISP_ERR_SHAPE;
   if (!isp::aligned16(q) || !isp::aligned16(out) || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
     return ISP_ERR_ALIGN;
   int64_t need = 0;
