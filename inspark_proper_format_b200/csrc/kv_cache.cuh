@@ -10,8 +10,8 @@
 // Token i of sequence b's n_b = cu[b + 1] - cu[b] tokens has position lengths[b] - n_b + i
 // (lengths counts the tokens of this call), found in page table[b][position / page_size].
 // A negative position means "no such token": nothing is written, zeros are read.  A
-// position past the page table or a page id outside the pool is recorded in the device
-// error word and treated the same way.
+// position past the page table, a page id outside the pool or counts outside the call's rows
+// are recorded in the device error word and treated the same way.
 #pragma once
 
 #include "common.cuh"
@@ -77,15 +77,18 @@ ISP_D int sequence_of(const int* cu, int batch, int64_t i) {
   return lo;
 }
 
-// Row (head 0) of packed token i, or -1.
-ISP_D int64_t row_of_token(const Cache& c, const Table& t, const int* cu, int64_t i) {
+// Whether [first, end) are rows of a call with `tokens` rows.
+ISP_D bool bounds_ok(int64_t first, int64_t end, int64_t tokens) { return first >= 0 && first <= end && end <= tokens; }
+
+// Row (head 0) of packed token i of `tokens`, or -1.
+ISP_D int64_t row_of_token(const Cache& c, const Table& t, const int* cu, int64_t i, int64_t tokens) {
   int b = static_cast<int>(i);
   int64_t first = i, end = i + 1;
   if (cu != nullptr) {
     b = sequence_of(cu, t.batch, i);
     first = cu[b];
     end = cu[b + 1];
-    if (i < first || i >= end) return -1;      // a token that no sequence claims
+    if (i < first || i >= end || !bounds_ok(first, end, tokens)) return -1;   // a token that no sequence claims
   }
   return row_of(c, t, b, static_cast<int>(t.lengths[b] - (end - first) + (i - first)));
 }
@@ -197,12 +200,16 @@ constexpr int kBoundsAtOnce = 1024;            // sequences whose bounds a block
 ISP_D int find_rows(const RowParams& p, int64_t first, int64_t (&rows)[kMaxTokensPerBlock], int (&bounds)[kBoundsAtOnce + 1]) {
   const int n = static_cast<int>(min(static_cast<int64_t>(p.tokens_per_block), p.tokens - first));
   const int* cu = p.cu;
+  if (cu != nullptr && blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < p.table.batch; i += kRowThreads)
+      if (!bounds_ok(cu[i], cu[i + 1], p.tokens)) record_bad_index();
+  }
   if (cu != nullptr && p.table.batch <= kBoundsAtOnce) {
     for (int i = threadIdx.x; i <= p.table.batch; i += kRowThreads) bounds[i] = p.cu[i];
     __syncthreads();
     cu = bounds;
   }
-  if (threadIdx.x < n) rows[threadIdx.x] = row_of_token(p.cache, p.table, cu, first + threadIdx.x);
+  if (threadIdx.x < n) rows[threadIdx.x] = row_of_token(p.cache, p.table, cu, first + threadIdx.x, p.tokens);
   __syncthreads();
   return n;
 }
