@@ -430,9 +430,10 @@ int isp_kv_append(const void *k, const void *v, int x_dtype, int64_t T,
                   const isp_kv_cache_t *cache, isp_stream_t stream);
 
 /* Read T rows back: code * scale (one FP32 product) rounded to out_dtype (ISP_BF16,
-   ISP_F16, ISP_F32).  k_out, v_out: [T, kv_heads, head_dim] contiguous.  With cu_seqlens
-   the running sum of `lengths` this unpages whole sequences, e.g. as the keys of
-   isp_prompt_attention. */
+   ISP_F16, ISP_F32).  k_out, v_out: [T, kv_heads, head_dim] contiguous; rows that no
+   sequence claims are zeros (all of them where B is 0; page_table and lengths may be NULL
+   then).  With cu_seqlens the running sum of `lengths` this unpages whole sequences, e.g. as
+   the keys of isp_prompt_attention. */
 int isp_kv_gather(const isp_kv_cache_t *cache, const int32_t *cu_seqlens,
                   const int32_t *page_table, int64_t table_stride, int table_width,
                   const int32_t *lengths, int B, int64_t T, int out_dtype,

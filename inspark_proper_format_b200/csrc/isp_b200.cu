@@ -1051,7 +1051,7 @@ int check_cache(const isp_kv_cache_t* c) {
 }
 
 int check_table(const int32_t* table, int64_t stride, int width, const int32_t* lengths, int B) {
-  if (table == nullptr || lengths == nullptr) return ISP_ERR_ARG;
+  if (B != 0 && (table == nullptr || lengths == nullptr)) return ISP_ERR_ARG;   // arrays of no element may be NULL
   if (B < 0 || width < 1 || stride < width) return ISP_ERR_SHAPE;
   return ISP_OK;
 }
@@ -1262,7 +1262,7 @@ int isp_kv_gather(const isp_kv_cache_t* cache, const int32_t* cu_seqlens, const 
   if (T < 0 || T >= kMaxTokens || (cu_seqlens == nullptr && T != B)) return ISP_ERR_SHAPE;
   if (!isp::aligned16(k_out) || !isp::aligned16(v_out)) return ISP_ERR_ALIGN;
   if (int st = isp::check_device()) return st;
-  if (T == 0 || B == 0) return ISP_OK;
+  if (T == 0) return ISP_OK;
   const int64_t head = cache->head_dim, token = head * cache->kv_heads;
   RowParams p{cache_of(*cache), {page_table, table_stride, table_width, lengths, B}, cu_seqlens, T,
               {static_cast<uint8_t*>(k_out), static_cast<uint8_t*>(v_out)}, {token, token}, {head, head},

@@ -82,6 +82,7 @@ ISP_D bool bounds_ok(int64_t first, int64_t end, int64_t tokens) { return first 
 
 // Row (head 0) of packed token i of `tokens`, or -1.
 ISP_D int64_t row_of_token(const Cache& c, const Table& t, const int* cu, int64_t i, int64_t tokens) {
+  if (t.batch == 0) return -1;
   int b = static_cast<int>(i);
   int64_t first = i, end = i + 1;
   if (cu != nullptr) {

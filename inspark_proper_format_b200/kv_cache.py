@@ -181,8 +181,7 @@ def kv_gather(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tens
         cu = index_array(cu_seqlens, "cu_seqlens", cache.device, batch + 1)
         if tokens is None or tokens < 0:
             raise ValueError("tokens must give the number of packed rows")
-    make = torch.empty if batch else torch.zeros
-    k, v = make((2, tokens, cache.kv_heads, cache.head_dim), device=cache.device, dtype=dtype).unbind(0)
-    if tokens and batch:
+    k, v = torch.empty((2, tokens, cache.kv_heads, cache.head_dim), device=cache.device, dtype=dtype).unbind(0)
+    if tokens:
         call(cache.device, "isp_kv_gather", cache.struct, cu, *table, tokens, _TYPES[dtype], k.data_ptr(), v.data_ptr())
     return k, v

@@ -76,3 +76,20 @@ def test_counts_inside_the_rows_are_not_recorded(kv, errors):
     k, _ = kv.kv_gather(cache, table, lengths, cu, tokens=12)
     assert errors() == 0
     assert k[:, 0, 0].tolist() == [0] * 2 + [1] * 7 + [0] * 3 and int(cache.k[:, 0, :, 0].sum()) == 4 + 3
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
+def test_rows_of_a_call_without_sequences_are_zeros(kv, errors, fmt):
+    """Nobody claims them: through the wrapper and the C entry, whose index arrays may be NULL then."""
+    from inspark_proper_format_b200 import _lib
+    cache = kv.PagedKVCache(2, 3, 64, page_size=16, fmt=fmt)
+    table, none, cu = torch.zeros(0, 2, dtype=torch.int32, device="cuda"), _i32([]), _i32([0])
+    rows = torch.ones(5, 3, 64, device="cuda").bfloat16()
+    kv.kv_append(cache, rows, rows, table, none, cu)
+    assert not cache.k.view(torch.uint8).any() and not cache.v.view(torch.uint8).any()
+    for got in kv.kv_gather(cache, table, none, cu, tokens=5):
+        assert got.shape == (5, 3, 64) and not got.any()
+    k, v = rows.clone(), rows.clone()
+    status = _lib.load().isp_kv_gather(ctypes.byref(cache._struct), cu.data_ptr(), None, 2, 2, None, 0, 5, _lib.BF16,
+                                       k.data_ptr(), v.data_ptr(), _lib.stream_handle())
+    assert status == _lib.ISP_OK and not k.any() and not v.any() and errors() == 0
