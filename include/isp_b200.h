@@ -449,7 +449,7 @@ int isp_kv_gather(const isp_kv_cache_t *cache, const int32_t *cu_seqlens,
  * q: [q_tokens, heads, head_dim], k, v: [k_tokens, kv_heads, head_dim] in `dtype` (ISP_BF16
  * or ISP_F16), out like q in the same type; strides in elements as in isp_kv_append.
  * cu_seqlens_q, cu_seqlens_k: int32 [B + 1] device arrays as above.  head_dim 64 or 128,
- * heads % kv_heads == 0, scale finite and positive, B <= 65536, fewer than 2^30 tokens,
+ * heads % kv_heads == 0, scale positive and scale * log2(e) finite, B <= 65536, fewer than 2^30 tokens,
  * k_tokens >= 1; strides of at least head_dim, and no two rows of `out` share an element
  * (ISP_ERR_SHAPE).
  */

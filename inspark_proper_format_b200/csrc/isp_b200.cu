@@ -1137,7 +1137,9 @@ int gather(const RowParams& p, int code, int out, unsigned grid, cudaStream_t s)
 
 namespace attn {
 
-bool scale_ok(float s) { return s > 0.f && s <= 3.402823466e38f; }
+constexpr float kLog2e = 1.44269504088896340736f;
+// the kernels take scale * log2(e)
+bool scale_ok(float s) { return s > 0.f && s * kLog2e <= 3.402823466e38f; }
 
 template <int kD, int kCode, int kType>
 int decode(const DecodeParams& p, cudaStream_t s) {
@@ -1318,7 +1320,7 @@ int isp_prompt_attention(const void* q, const void* k, const void* v, int dtype,
   p.batch = B;
   p.heads = heads;
   p.group = heads / kv_heads;
-  p.scale = scale * 1.44269504088896340736f;
+  p.scale = scale * isp::attn::kLog2e;
   p.causal = causal;
   p.out32 = (reinterpret_cast<uintptr_t>(out) % 32 == 0 && out_token_stride % 16 == 0 && out_head_stride % 16 == 0) ? 1 : 0;
   if (head_dim == 64)
@@ -1367,7 +1369,7 @@ int isp_paged_decode(const void* q, int dtype, int64_t q_seq_stride, int64_t q_h
   p.group = heads / cache->kv_heads;
   p.gblocks = (p.group + 7) / 8;
   p.gb = p.group < 8 ? p.group : 8;
-  p.scale = scale * 1.44269504088896340736f;
+  p.scale = scale * isp::attn::kLog2e;
   p.counters = static_cast<unsigned*>(workspace);
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + isp::attn::kMaxBlocks * 4);
   return cache->head_dim == 64 ? isp::attn::decode_type<64>(p, dtype, cache->dtype, stream)

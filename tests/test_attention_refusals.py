@@ -45,3 +45,12 @@ def test_output_rows_that_overlap_are_refused(lib, entry, tokens, heads):
                 status = entry(lib, tokens, heads, dim, (token_stride, head_stride))
                 want = 1 if _overlap(tokens, heads, dim, token_stride, head_stride) else 2
                 assert status == want, (token_stride, head_stride)
+
+
+@pytest.mark.parametrize("entry", [_prompt, _decode])
+def test_scales_that_overflow_in_base_2_are_refused(lib, entry):
+    """The kernels take scale * log2(e), which is infinite from FP32's largest value / 1.4427 on."""
+    for scale in (2.4e38, 3.4e38, float("inf"), 0.0, -1.0, float("nan")):
+        assert entry(lib, scale=scale) == 7, scale
+    for scale in (2.3e38, 1e-40, 1.0):
+        assert entry(lib, scale=scale) == 2, scale
