@@ -2,7 +2,9 @@
 //
 // o_i = sum_j p_ij v_j / sum_j p_ij over the keys j that query i sees, p_ij =
 // 2^(scale log2(e) q_i.k_j - m_i), with the running maximum m and sum of each row in FP32,
-// one pass over K and V.
+// one pass over K and V.  p enters the product with V in the operands' type: BF16, or FP16 times
+// 2^7, which keeps all its bits down to 2^-21 of a row's largest weight and loses what lies below
+// 2^-32 of it (FP16 rows reach from 2^-24 to 2^16).
 //
 // A work item is a block of 256 queries of one (sequence, head): two tiles of 128 that share
 // every K and V tile of 128 keys.  Blocks of the grid are persistent and take items in an
@@ -589,6 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;        // TMEM lane quarter
     const uint32_t s_tmem = tmem + L::s(t) + lanes, o_tmem = tmem + L::o(t) + lanes;
     const float slack = kSlack / p.scale;
+    constexpr float kPlace = kBf16 ? 0.f : 15.f - kSlack;                // FP16 weights as high as FP16 allows
     uint32_t s_count = 0, o_count = 0, turns = 0;                        // turns: of the other tile, in the items before
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
@@ -602,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       const int sees = static_cast<int>(min(static_cast<int64_t>(it.keys), static_cast<int64_t>(it.off) + row + 1));
       const int whole = min(it.keys, it.off + first + 1);
       const bool take_turns = min(steps, steps_other) >= kTurnSteps;
-      float m = -INFINITY, shift = 0.f, base = 0.f;                      // m in units of q.k
+      float m = -INFINITY, shift = 0.f, base = -kPlace;                      // m in units of q.k
       bool far = false;
       float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = 0; j < steps; ++j) {
@@ -647,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           // count (scores beyond 2^16), the difference is taken first
           shift = m == -INFINITY ? 0.f : m;
           far = __any_sync(0xffffffffu, fabsf(shift * p.scale) > 65536.f);
-          base = far ? 0.f : shift * p.scale;
+          base = (far ? 0.f : shift * p.scale) - kPlace;
         }
         if (far) {
 #pragma unroll

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from attention_f64 import attend, check
+from attention_f64 import U, attend, bound
 from test_gpu_attention import _cu, _i32, _randn, check_decode, make_cache
 from test_gpu_kv_cache import layout
 
@@ -81,3 +81,51 @@ def test_decode_value_rows_over_32_octaves(at, kv, order, fmt):
     v *= torch.exp2(octaves.round())[:, None, None].cuda()
     cache, table, back = cache_of(kv, k, v, lens, 64, fmt, 114)
     check_decode(at.paged_decode_attention(q, cache, table, _i32(lens)), q, back, lens)
+
+
+def fp16_rows(n, heads, kv_heads, dim, seed):
+    """q, k, v of n tokens: key j's weight is about 2^-drop_j of the first key's, its values 2^drop_j
+    of the first's, drop_j from 0 to 26, so all keys count alike."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    drop = torch.randint(0, 27, (n, kv_heads, 1), device="cuda", generator=g).float()
+    drop[0] = 0
+    q = _randn(n, heads, dim, seed=seed + 1, dtype=torch.float16, gain=0.1)
+    q[..., 0] = 1.0
+    k = _randn(n, kv_heads, dim, seed=seed + 2, dtype=torch.float16, gain=0.1)
+    k[..., :1] = -drop * np.log(2.0) * dim ** 0.5
+    v = (0.5 + 0.5 * torch.rand(n, kv_heads, dim, device="cuda", generator=g)) * torch.exp2(drop - 12)
+    return q, k, v.half()
+
+
+def check_fp16(got, q, k, v, causal):
+    """The bound of attention_f64, and what FP16's smallest steps add: the largest weight of a row is
+    at least 2^7 units, so rounding to multiples of 2^-24 units is off by at most 2^-32 of it."""
+    n, heads, dim = q.shape
+    out, size, spread = attend(q, k, v, dim ** -0.5, causal)
+    group = heads // k.shape[1]
+    s = torch.einsum("qhd,khd->hqk", q.double(), k.double().repeat_interleave(group, 1)) * dim ** -0.5
+    seen = torch.ones_like(s, dtype=torch.bool)
+    if causal:
+        seen = seen.tril(k.shape[0] - n)
+    s = s.masked_fill(~seen, -torch.inf)
+    total = torch.exp(s - s.amax(-1, keepdim=True)).sum(-1).transpose(0, 1)[..., None]
+    steps = torch.einsum("hqk,khd->qhd", seen.double(), v.double().abs().repeat_interleave(group, 1)) * 2.0 ** -32 / total
+    err = (got.double() - out).abs()
+    lim = bound(out, size, spread, torch.float16, dim, U[torch.float16]) + steps
+    assert bool((err <= lim).all()), f"worst {float((err / lim).max()):.3g} x bound"
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [40, 700])
+def test_prompt_fp16_small_weights_of_large_values(at, n, dim, causal):
+    q, k, v = fp16_rows(n, 4, 2, dim, 130)
+    check_fp16(at.prompt_attention(q, k, v, _cu([n]), causal=causal), q, k, v, causal)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [40, 5000])
+def test_decode_fp16_small_weights_of_large_values(at, kv, n, dim):
+    q, k, v = fp16_rows(n, 4, 2, dim, 140)
+    cache, table, _ = cache_of(kv, k, v, [n], 16, "f16", 141)
+    check_fp16(at.paged_decode_attention(q[-1:], cache, table, _i32([n])), q[-1:], k, v, False)
