@@ -443,15 +443,16 @@ int isp_kv_gather(const isp_kv_cache_t *cache, const int32_t *cu_seqlens,
  * Attention of packed sequences: out = softmax(scale * q k^T) v per sequence and head,
  * query head h with key head h / (heads / kv_heads).  Query i of sequence b's n sees its m
  * keys all (causal = 0) or keys j <= i + m - n (causal = 1: the last query sees the last
- * key); a query that sees no key gets zeros.  Masked keys and values are not read into the
- * result whatever they hold.
+ * key); a query that sees no key, or only keys with a score of -infinity, gets zeros, one with a
+ * score of +infinity or NaN gets NaN.  Masked keys and values are not read into the result
+ * whatever they hold.
  *
  * q: [q_tokens, heads, head_dim], k, v: [k_tokens, kv_heads, head_dim] in `dtype` (ISP_BF16
  * or ISP_F16), out like q in the same type; strides in elements as in isp_kv_append.
  * cu_seqlens_q, cu_seqlens_k: int32 [B + 1] device arrays as above.  head_dim 64 or 128,
- * heads % kv_heads == 0, scale positive and scale * log2(e) finite, B <= 65536, fewer than 2^30 tokens,
- * k_tokens >= 1; strides of at least head_dim, and no two rows of `out` share an element
- * (ISP_ERR_SHAPE).
+ * heads % kv_heads == 0, scale positive and scale * log2(e) finite, B <= 65536, fewer than
+ * 2^30 tokens, k_tokens >= 1; strides of at least head_dim, and no two rows of `out` share an
+ * element (ISP_ERR_SHAPE).
  */
 int isp_prompt_attention(const void *q, const void *k, const void *v, int dtype,
                          int64_t q_tokens, int64_t k_tokens,
@@ -467,8 +468,9 @@ int isp_prompt_attention(const void *q, const void *k, const void *v, int dtype,
 /*
  * Attention of one token per sequence over the paged cache: q, out: [B, heads, head_dim] in
  * `dtype` (ISP_BF16 or ISP_F16), strides as above; the token sees positions
- * [0, lengths[b]) (its own row is appended before); length 0 gives zeros.  A 16-bit cache
- * has q's type.  B <= 65535; no two rows of `out` share an element (ISP_ERR_SHAPE).
+ * [0, lengths[b]) (its own row is appended before); length 0 gives zeros, infinite scores what
+ * they give above.  A 16-bit cache has q's type.  B <= 65535; no two rows of `out` share an
+ * element (ISP_ERR_SHAPE).
  *
  * workspace: isp_paged_decode_workspace bytes of device memory, 256-byte aligned, zero
  * before its first use; every call leaves it ready for the next one on the same stream.

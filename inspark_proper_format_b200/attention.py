@@ -47,8 +47,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     the same) of k and v.
 
     Causal attention is aligned at the end: query i of n sees keys ``j <= i + m - n`` of m,
-    so the queries may follow a cached prefix.  A query that sees no key gives zeros; rows
-    that no sequence claims are undefined.  ``scale`` defaults to ``1 / sqrt(dim)``."""
+    so the queries may follow a cached prefix.  A query that sees no key, or only keys with a
+    score of -inf, gives zeros; rows that no sequence claims are undefined.  ``scale`` defaults
+    to ``1 / sqrt(dim)``."""
     if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
         raise ValueError("expected q [tokens, heads, dim] and k, v [keys, kv_heads, dim]")
     if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
