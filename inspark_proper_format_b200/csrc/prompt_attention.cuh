@@ -665,11 +665,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         for (int c = 0; c < 4; ++c) {                                    // p replaces the scores
           chunk_weights<kBf16>(x[c], p.scale, base, l, s_tmem + c * 16);
           if (c == 2 && lane == 0) atomicAdd(&bars.turn[t], 1u);     // the last quarter may overlap
+          __syncwarp();
           if (c >= 2) {                                                  // half a tile, a chunk later
             tmem_st_wait();
             gemm::tc_fence_before();
             __syncwarp();
             if (lane == 0) gemm::mbar_arrive(&bars.p_full[t][c - 2]);
+            __syncwarp();
           }
         }
         if (!(top < INFINITY)) l[0].x = __int_as_float(0x7fc00000);      // a NaN or an infinite score: the row is NaN
@@ -701,22 +703,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (!mine) continue;
-        uint32_t w[16];
+        if (mine) {
+          uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = pack<kBf16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-        if (p.out32) {
+          for (int i = 0; i < 16; ++i) w[i] = pack<kBf16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          if (p.out32) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c * 64 + i * 32),
-                         "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]), "r"(w[8 * i + 4]),
-                         "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
-                         : "memory");
-        } else {
+            for (int i = 0; i < 2; ++i)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c * 64 + i * 32),
+                           "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]), "r"(w[8 * i + 4]),
+                           "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
+                           : "memory");
+          } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(dst + c * 64 + i * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(dst + c * 64 + i * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          }
         }
+        __syncwarp();                                                    // the next read of TMEM is the whole warp's
       }
       if (steps > 0 && mine && *reinterpret_cast<const volatile int*>(&it.flagged) != 0) {
         // what the V check set to zero and this row sees: infinities and NaN, which take the element over
