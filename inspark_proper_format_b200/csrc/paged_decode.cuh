@@ -26,17 +26,18 @@
 // 16 bytes it loads as its fragment, with keys in the order of key_row() that makes K's
 // rows V's columns and keeps both reads free of bank conflicts.  Their scales go to the
 // FP32 scores (K) and to p (V): p * v_scale carries a power of two that follows its largest
-// value so far and keeps that between 2^6 and 2^15, so FP16 has all its bits down to 2^-20 of
-// the largest p * v_scale and loses what lies below 2^-31 of it.  BF16 queries over 8-bit rows
-// are brought into FP16's range by a power of two per head and keep all their bits down to
-// 2^-31 of the head's largest element; below 2^-39 of it they are lost.  p is rounded once to 16
-// bits: FP16 over 8-bit and FP16 rows (over the latter p times 2^7, all bits down to 2^-21 of the
-// largest weight, lost below 2^-32), BF16 over BF16 rows; sums are FP32.
+// value so far and keeps that between 2^6 and 2^15.  BF16 queries over 8-bit rows are brought
+// into FP16's range by a power of two per head and keep all their bits down to 2^-31 of the
+// head's largest element; below 2^-39 of it they are lost.  p is rounded to 16 bits: FP16 over
+// 8-bit and FP16 rows (over the latter p times 2^7), BF16 over BF16 rows.  What FP16 cannot hold
+// of a small weight goes into a second product, so weights keep the result's bits down to 2^-60
+// of the largest (it costs 3% on the E4M3 case below, 7% on the INT8 case, whose scores spread
+// so far that half of the 16-key blocks have such weights).  Sums are FP32.
 //
 // Measured on one B200, cold inputs: INT8, head_dim 128, 32 over 8 heads, 238651 cached
-// tokens 100 us (5.0 TB/s); FP16, the same heads, 37 sequences of up to 6000 tokens 29.0 us
-// (3.27 TB/s); E4M3, head_dim 64, 20 heads, 64 sequences of 256 to 2048 tokens 44.9 us
-// (3.38 TB/s), bound by latency in the warps' unpacking rather than by the copies, which
+// tokens 106 us (4.8 TB/s); FP16, the same heads, 37 sequences of up to 6000 tokens 29.2 us
+// (3.24 TB/s); E4M3, head_dim 64, 20 heads, 64 sequences of 256 to 2048 tokens 46.4 us
+// (3.27 TB/s), bound by latency in the warps' unpacking rather than by the copies, which
 // alone take 29 us.
 #pragma once
 
@@ -411,6 +412,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
   // - 1), 2^15], whatever the scales of rows are whose own weight is small.  Either reference may
   // stay up to kSlack behind, so that most tiles rescale nothing.
   constexpr float kSlack = 8.f, kUp = 15.f - kSlack;
+  // Below 2^-17 (2^-14) FP16 has fewer bits than the result's 8 (11): the bits of that limit
+  constexpr unsigned kSmall = kQBf16 ? 0x37000000u : 0x38800000u;
+  constexpr float kRestUnits = 0x1p40f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, r[2] = {-INFINITY, -INFINITY}, c[2] = {0.f, 0.f};
   // log2 of |v_scale|, rounded up; scales under 2^-64 are not brought up
   const auto log2_above = [](float v) { return fmaxf(static_cast<float>(static_cast<int>((__float_as_uint(v) >> 23) & 255u) - 126), -64.f); };
@@ -570,17 +574,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
     const float base[2] = {(m[0] == -INFINITY ? 0.f : m[0]) - kPlace, (m[1] == -INFINITY ? 0.f : m[1]) - kPlace};
 
     // ---- weights and their product with V, 16 keys at a time ----
-#pragma unroll
-    for (int kb = 0; kb < kKeyBlocks; ++kb) {
-      float w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j] = exp2_approx(s[kb][j] - base[j & 1]);
-        l[j & 1] += w[j];
-        if constexpr (kIsCode) w[j] = w[j] * c[j & 1] * f[kb][j >> 1].y;
-      }
-      const uint32_t b0 = transpose8x8(pack16<kMmaBf16>(w[0], w[1]));
-      const uint32_t b1 = transpose8x8(pack16<kMmaBf16>(w[2], w[3]));
+    // V's fragments of key block kb, one for every 16 head dimensions, to `use`
+    const auto each_v = [&](int kb, const auto& use) {
       if constexpr (kIsCode) {
         // this lane's kD / 8 elements of each row: kD / 8 * g ..; row g of output block j takes
         // element 2j, row g + 8 element 2j + 1
@@ -603,14 +598,44 @@ __global__ void __launch_bounds__(kDecWarps * 32, Tile<kD, kCode>::kBlocks) deco
           Frag v;
           codes_to_f16<kCode>(prmt(x[0][j / 2], x[1][j / 2], sel), v[0], v[1]);
           codes_to_f16<kCode>(prmt(x[2][j / 2], x[3][j / 2], sel), v[2], v[3]);
-          mma16816<false>(o[j], v, b0, b1);
+          use(j, v);
         }
       } else {
 #pragma unroll
         for (int j = 0; j < kOBlocks; ++j) {
           const int r = kb * 16 + lv_row;
-          const Frag v = ldmatrix4<true>(st_u32 + T::kV + r * kRow + (((2 * j + lv_chunk) ^ (lane & 7)) << 4));
-          mma16816<kMmaBf16>(o[j], v, b0, b1);
+          use(j, ldmatrix4<true>(st_u32 + T::kV + r * kRow + (((2 * j + lv_chunk) ^ (lane & 7)) << 4)));
+        }
+      }
+    };
+#pragma unroll
+    for (int kb = 0; kb < kKeyBlocks; ++kb) {
+      float w[4];
+      unsigned least = 0xFFFFFFFFu;                    // of the weights' bits, minus 1, so that 0 counts as large
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = exp2_approx(s[kb][j] - base[j & 1]);
+        l[j & 1] += w[j];
+        if constexpr (kIsCode) w[j] = w[j] * c[j & 1] * f[kb][j >> 1].y;
+        least = min(least, __float_as_uint(w[j]) - 1u);
+      }
+      const uint32_t p01 = pack16<kMmaBf16>(w[0], w[1]), p23 = pack16<kMmaBf16>(w[2], w[3]);
+      const uint32_t b0 = transpose8x8(p01), b1 = transpose8x8(p23);
+      each_v(kb, [&](int j, const Frag& v) { mma16816<kMmaBf16>(o[j], v, b0, b1); });
+      if constexpr (!kMmaBf16) {
+        if (__any_sync(0xffffffffu, least < kSmall - 1u)) {
+          // The rounding left at most 2^-25 of a small weight.  It counts where the rows with the
+          // larger products are 0, so it is added in a second product, in units of 2^-40.
+          const auto left = [&](float x, float rounded) { return __float_as_uint(x) < kSmall ? (x - rounded) * kRestUnits : 0.f; };
+          const float2 r01 = unpack16<false>(p01), r23 = unpack16<false>(p23);
+          const uint32_t c0 = transpose8x8(pack16<false>(left(w[0], r01.x), left(w[1], r01.y)));
+          const uint32_t c1 = transpose8x8(pack16<false>(left(w[2], r23.x), left(w[3], r23.y)));
+          each_v(kb, [&](int j, const Frag& v) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            mma16816<false>(x, v, c0, c1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[j][i] = fmaf(x[i], 1.f / kRestUnits, o[j][i]);
+          });
         }
       }
     }

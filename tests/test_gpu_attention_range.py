@@ -129,3 +129,39 @@ def test_decode_fp16_small_weights_of_large_values(at, kv, n, dim):
     q, k, v = fp16_rows(n, 4, 2, dim, 140)
     cache, table, _ = cache_of(kv, k, v, [n], 16, "f16", 141)
     check_fp16(at.paged_decode_attention(q[-1:], cache, table, _i32([n])), q[-1:], k, v, False)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [2, 300])
+def test_decode_small_rows_where_the_large_are_zero(at, kv, n, dim, fmt):
+    """Every other row is 2^up larger, and zero in the odd elements, which the small rows alone make."""
+    q = _randn(3, 4, dim, seed=170, dtype=torch.bfloat16)
+    k = _randn(n, 2, dim, seed=171, dtype=torch.float32)
+    even = (torch.arange(dim, device="cuda") % 2 == 0).float()
+    for up in (20, 32, 45, 58):
+        v = _randn(n, 2, dim, seed=172, dtype=torch.float32)
+        v[0::2] *= 2.0 ** up * even
+        v[1::2] *= 1 - even
+        cache, table, back = cache_of(kv, k, v, [n], 16, fmt, 173)
+        for row in range(3):
+            check_decode(at.paged_decode_attention(q[row:row + 1], cache, table, _i32([n])), q[row:row + 1], back, [n])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "f16"])
+@pytest.mark.parametrize("n", [2, 300])
+def test_decode_fp16_small_weights_where_the_large_rows_are_zero(at, kv, n, fmt):
+    """Every other key has 2^-drop of the weight, and the odd elements of V to itself."""
+    dim = 64
+    q = _randn(1, 4, dim, seed=180, dtype=torch.float16, gain=0.1)
+    q[..., 0] = 1.0
+    even = (torch.arange(dim, device="cuda") % 2 == 0).float()
+    for drop in (26, 31, 34, 37):
+        k = _randn(n, 2, dim, seed=181, dtype=torch.float32) * 0.1
+        k[..., 0] = 0
+        k[1::2, :, 0] = -drop * np.log(2.0) * dim ** 0.5
+        v = 1.0 + torch.rand(n, 2, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(182))
+        v[0::2] *= even
+        v[1::2] *= (1 - even) * 2.0 ** 14
+        cache, table, back = cache_of(kv, k.half(), v.half(), [n], 16, fmt, 183)
+        check_decode(at.paged_decode_attention(q, cache, table, _i32([n])), q, back, [n])
