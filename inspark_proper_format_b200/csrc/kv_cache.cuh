@@ -250,9 +250,9 @@ struct RowWalk {
 // BF16 rows 33.3 us, 37.5 in such blocks); gather, with less work a row, four waves, so that
 // some blocks look up while others move (2% faster than blocks of 256 rows, 7% than one
 // wave).  One row a lane at a time: two or four in flight cost registers, and with them more
-// than they hid (10 and 45%).  Measured, append then gather on one B200: INT8, 64 x 256
-// tokens, 20 heads of 64, 59.5 us (4.3 TB/s of 257 MB); E4M3, 44246 tokens, 8 heads of 128,
-// 110 us (5.0 TB/s of 549 MB).
+// than they hid (10 and 45%).  Measured, append then gather on one B200, launches of a captured
+// graph over changing inputs: INT8, 64 x 256 tokens, 20 heads of 64, 58.7 us (4.4 TB/s of 257
+// MB); E4M3, 44246 tokens, 8 heads of 128, 109 us (5.0 TB/s of 549 MB), as calls 115 us.
 template <int kD, int kIn, int kCode>
 __global__ void __launch_bounds__(kRowThreads, append_blocks(kCode)) append_kernel(const RowParams p) {
   constexpr int kElems = is_code(kCode) ? 16 : 8, kLanes = kD / kElems;

@@ -31,14 +31,14 @@
 // head's largest element; below 2^-39 of it they are lost.  p is rounded to 16 bits: FP16 over
 // 8-bit and FP16 rows (over the latter p times 2^7), BF16 over BF16 rows.  What FP16 cannot hold
 // of a small weight goes into a second product, so weights keep the result's bits down to 2^-60
-// of the largest (it costs 3% on the E4M3 case below, 7% on the INT8 case, whose scores spread
-// so far that half of the 16-key blocks have such weights).  Sums are FP32.
+// of the largest.  (It costs 3% on the E4M3 case below, where few blocks of 16 keys have such
+// weights, and 7% on the INT8 case, where a third have.)  Sums are FP32.
 //
-// Measured on one B200, cold inputs: INT8, head_dim 128, 32 over 8 heads, 238651 cached
-// tokens 106 us (4.8 TB/s); FP16, the same heads, 37 sequences of up to 6000 tokens 29.2 us
-// (3.24 TB/s); E4M3, head_dim 64, 20 heads, 64 sequences of 256 to 2048 tokens 46.4 us
-// (3.27 TB/s), bound by latency in the warps' unpacking rather than by the copies, which
-// alone take 29 us.
+// Measured on one B200, launches of a captured graph over changing inputs: INT8, head_dim 128,
+// 32 over 8 heads, 238651 cached tokens 106 us (4.8 TB/s; as calls 115 us); FP16, the same heads,
+// 37 sequences of up to 6000 tokens 29.2 us (3.24 TB/s); E4M3, head_dim 64, 20 heads, 64
+// sequences of 256 to 2048 tokens 46.4 us (3.27 TB/s), bound by latency in the warps' unpacking
+// rather than by the copies, which alone take 29 us.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -171,7 +171,9 @@ struct Tile {
   static constexpr int kChunks = kRow / 16;
   static constexpr int kStep = kDecWarps * kT;             // positions of one unit of work
   // Ring depth and blocks per SM: 16 warps with two 4 KB tiles each in flight, or 12 with one
-  // of 8 KB (three stages for two blocks, or 16-row tiles, are 2 to 10% slower).
+  // of 8 KB (three stages for two blocks, or 16-row tiles, are 2 to 10% slower).  The joins leave
+  // room for a block less from 4 query heads to a key head on (codes), 5 (16-bit rows, head_dim
+  // 128) or 8 (head_dim 64).
   static constexpr int kStages = kRow == 64 ? 3 : 2;
   static constexpr int kBlocks = kRow == 64 ? 4 : 3;
   // stage: K rows, V rows, per row {K scale, V scale}, the valid mask

@@ -25,18 +25,22 @@
 //                   rows at the end.
 // Every wait is bounded; on expiry the block unwinds as the GEMMs do.
 //
-// Measured on one B200: 16384 tokens, 32 over 8 heads of 128, 2.04 ms call after call (at the
-// power cap; 1.08 PFLOP/s of causal work) and 1.78 ms alone; 64 x 760 frames, 8 heads of 64,
-// every key, 139 us; 64 x 256 tokens, 20 heads of 64, 55.7 us.  Bound by the softmax: a step of
-// both tiles takes about 3800 cycles, of them 2048 in the special function unit and as many in
-// the tensor pipe (each busy for 0.6 of the time); what is left is the chain S -> maximum ->
-// exponentials -> PV of a tile.  Tried and slower: half of the exponentials or fewer by
-// polynomial (5 to 25%, the warps are bound by their own instruction chains), a second read of
-// S in a rolled loop (15%; for masked tiles alone 3 to 7%), two threads a row (5 to 20% on long
-// items), half of S(j + 1) before PV(j) (4%), no turns (10 to 18%).  The roles' code has to stay
-// small, they share the instruction cache: rolling the output and the repair of non-finite
-// values alone took 3 to 8% off, two scores to an instruction (f32x2) in the products and sums
-// of the exponentials another 3 to 9%.
+// Measured on one B200, launches of a captured graph over changing inputs (and calls among
+// others): 16384 tokens, 32 over 8 heads of 128, 2.04 ms (2.10 ms; both at the power cap, 1.08
+// PFLOP/s of causal work; a single launch 1.8 to 1.9 ms); 64 x 760 frames, 8 heads of 64, every key,
+// 139 us (156 us); 64 x 256 tokens, 20 heads of 64, 56.2 us (57.1 us).  Bound by the chain S ->
+// maximum -> exponentials -> PV -> next S of a tile (P lies over S): a step of both tiles of the
+// long case takes about 3800 cycles, of them 2048 in the special function unit and as many in the
+// tensor pipe, each busy for 0.6 of the time; over the frames they are for 0.52 and 0.32.  Finding
+// an item scans the sequences' bounds a few times, which shows from about a thousand short
+// sequences on (8192 sequences of 1 to 64 tokens, 8 heads: 11 ms, 512 of them 137 us).
+// Tried and slower: half of the exponentials or fewer by polynomial (5 to 25%, the warps are
+// bound by their own instruction chains), a second read of S in a rolled loop (15%; for masked
+// tiles alone 3 to 7%), two threads a row (5 to 20% on long items), half of S(j + 1) before PV(j),
+// P over S all the same (4%), no turns (10 to 18%).  The roles' code has to stay small, they share
+// the instruction cache: rolling the output and the repair of non-finite values alone took 3 to
+// 8% off, two scores to an instruction (f32x2) in the products and sums of the exponentials
+// another 3 to 9%.
 #pragma once
 
 #include "gemm_sm100.cuh"
