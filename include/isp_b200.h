@@ -452,7 +452,7 @@ int isp_kv_gather(const isp_kv_cache_t *cache, const int32_t *cu_seqlens,
  * cu_seqlens_q, cu_seqlens_k: int32 [B + 1] device arrays as above.  head_dim 64 or 128,
  * heads % kv_heads == 0, scale positive and scale * log2(e) finite, B <= 65536, fewer than
  * 2^30 tokens, k_tokens >= 1; strides of at least head_dim, and no two rows of `out` share an
- * element (ISP_ERR_SHAPE).
+ * element (ISP_ERR_SHAPE).  `out` shares no memory with q, k and v.
  */
 int isp_prompt_attention(const void *q, const void *k, const void *v, int dtype,
                          int64_t q_tokens, int64_t k_tokens,
@@ -470,7 +470,7 @@ int isp_prompt_attention(const void *q, const void *k, const void *v, int dtype,
  * `dtype` (ISP_BF16 or ISP_F16), strides as above; the token sees positions
  * [0, lengths[b]) (its own row is appended before); length 0 gives zeros, infinite scores what
  * they give above.  A 16-bit cache has q's type.  B <= 65535; no two rows of `out` share an
- * element (ISP_ERR_SHAPE).
+ * element (ISP_ERR_SHAPE), and `out` shares no memory with q and the cache.
  *
  * workspace: isp_paged_decode_workspace bytes of device memory, 256-byte aligned, zero
  * before its first use; every call leaves it ready for the next one on the same stream.
